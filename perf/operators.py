@@ -1,0 +1,314 @@
+"""Performance cases of the operators for expert models, their tuning by rewards and their serving in 8 bits.
+
+    experts   products of ragged groups of rows, each with its expert's weights: forward, or forward and backward
+    fp8       product in 8-bit floating point with a scale for each block of 128, activations quantised within the call;
+              dense, or over ragged groups of rows as in `experts`
+    policy    clipped policy loss with a KL term over a vocabulary, forward and backward
+
+A case is a dict with a "kind" and its sizes.  `listed()` gives the fixed set, `draw(rng)` one more case of the same ranges,
+`prepare` what the program has in hand before the call, `run` one pass (with `own` through the package, without it by elementary
+tensor operations in 32 bits), `work` the bytes and operations a pass cannot do without, `exact` the same outputs in 64 bits.
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import torch
+
+own = False
+
+BLOCK = 128                       # values that share a scale
+E4M3_MAX = 448.0
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+CLIP = (0.2, 0.28)                # how far below and above one the ratio may go
+KL = 0.04
+
+MAX_PRODUCT = 16384 * 2048 * 5504           # tokens x hidden x ffn of the largest expert layer
+MAX_EXPERTS = 32 * 2048 * 5504              # weights of all its experts
+MAX_FP8 = 8192 * 8192 * 3584
+MAX_LOGITS = 8192 * 50304
+
+
+def listed():
+    return [
+        # One token of a decoder that sends every token to two experts: the latency of a call, two of eight weights read.
+        {"name": "experts_one_token", "kind": "experts", "tokens": 2, "experts": 8, "hidden": 1024, "ffn": 2048, "train": False, "skew": 0.0},
+        # Sampling with a batch: a row or two for each of many experts, every weight read once.
+        {"name": "experts_batch", "kind": "experts", "tokens": 64, "experts": 32, "hidden": 2048, "ffn": 5504, "train": False, "skew": 0.3},
+        # The expert layer of the repository's benchmark case in training, without slots: all tokens are kept, however uneven.
+        {"name": "experts_8", "kind": "experts", "tokens": 8192, "experts": 8, "hidden": 1024, "ffn": 2048, "train": True, "skew": 0.5},
+        # Many small experts of odd sizes on an uneven batch, some without a token.
+        {"name": "experts_ragged", "kind": "experts", "tokens": 3001, "experts": 64, "hidden": 520, "ffn": 776, "train": True, "skew": 1.5},
+        # A large training batch at the widths of the decoder in training (perf/cases.py).
+        {"name": "experts_large", "kind": "experts", "tokens": 16384, "experts": 8, "hidden": 2048, "ffn": 5504, "train": True, "skew": 0.3},
+        # One sequence being sampled: a single row through the decoder's default up projection.
+        {"name": "fp8_one_row", "kind": "fp8", "rows": 1, "experts": 0, "k": 4096, "n": 11008, "skew": 0.0},
+        # A batch of sequences being sampled, through a down projection.
+        {"name": "fp8_batch", "kind": "fp8", "rows": 48, "experts": 0, "k": 8192, "n": 3584, "skew": 0.0},
+        # Prefill at the sizes of the bf16 product's benchmark.
+        {"name": "fp8_prefill", "kind": "fp8", "rows": 8192, "experts": 0, "k": 8192, "n": 3584, "skew": 0.0},
+        # Prefill through experts, the last block of 128 of a row not full.
+        {"name": "fp8_experts", "kind": "fp8", "rows": 5003, "experts": 16, "k": 2064, "n": 5504, "skew": 0.5},
+        # A unit test's or a small model's loss: latency.
+        {"name": "policy_short", "kind": "policy", "rows": 96, "vocab": 1000, "padded": False, "dtype": "bf16", "kl": True, "mean": True},
+        # The tokens of a training step over the benchmark's vocabulary, padded to a multiple of 64 columns.
+        {"name": "policy_8192", "kind": "policy", "rows": 8192, "vocab": 50257, "padded": True, "dtype": "bf16", "kl": True, "mean": True},
+        # A wide vocabulary, logits kept in 32 bits, summed (the caller divides by the tokens of all ranks).
+        {"name": "policy_wide", "kind": "policy", "rows": 1500, "vocab": 131072, "padded": False, "dtype": "fp32", "kl": False, "mean": False},
+    ]
+
+
+# ---- drawing --------------------------------------------------------------------------------------------------------
+def _log_int(rng, lo, hi, step=1):
+    """A multiple of `step` in [lo, hi], uniform in its logarithm."""
+    v = math.exp(rng.uniform(math.log(lo), math.log(hi)))
+    return max(lo, min(hi // step * step, int(round(v / step)) * step))
+
+
+def draw(rng):
+    kind = rng.choice(["experts", "experts", "fp8", "fp8", "policy"])
+    if kind == "experts":
+        hidden, ffn, experts = _log_int(rng, 64, 2048, 8), _log_int(rng, 64, 5504, 8), _log_int(rng, 1, 64)
+        experts = max(1, min(experts, MAX_EXPERTS // (hidden * ffn)))
+        return {"kind": kind, "tokens": _log_int(rng, 1, min(16384, MAX_PRODUCT // (hidden * ffn))), "experts": experts, "hidden": hidden,
+                "ffn": ffn, "train": rng.random() < 0.6, "skew": rng.choice([0.0, 0.3, 1.0, 2.0])}
+    if kind == "fp8":
+        k, n, experts = _log_int(rng, 128, 8192, 16), _log_int(rng, 64, 11008, 8), rng.choice([0, 0, 4, 8, 16, 64])
+        if experts:
+            experts = max(1, min(experts, MAX_EXPERTS // (k * n)))
+        return {"kind": kind, "rows": _log_int(rng, 1, min(8192, MAX_FP8 // (k * n))), "experts": experts, "k": k, "n": n,
+                "skew": rng.choice([0.0, 0.3, 1.0])}
+    vocab, dtype = _log_int(rng, 64, 131072), rng.choice(["bf16", "bf16", "fp16", "fp32"])
+    most = MAX_LOGITS // (2 if dtype == "fp32" else 1) // (vocab + 63)
+    return {"kind": kind, "rows": _log_int(rng, 1, min(16384, most)), "vocab": vocab, "padded": rng.random() < 0.5, "dtype": dtype,
+            "kl": rng.random() < 0.6, "mean": rng.random() < 0.6}
+
+
+# ---- what the program has in hand -----------------------------------------------------------------------------------
+def _group_sizes(tokens, experts, skew, seed):
+    """How many rows each expert gets: shares spread by exp(skew x normal), or top-k's distinct experts for a few rows."""
+    rng = random.Random(seed)
+    share = [math.exp(skew * rng.gauss(0, 1)) for _ in range(experts)]
+    if tokens < 4 * experts:                                     # few rows: drawn one by one
+        picked = rng.choices(range(experts), share, k=tokens)
+        return [picked.count(e) for e in range(experts)]
+    total, run, cuts = sum(share), 0.0, [0]
+    for s in share:
+        run += s
+        cuts.append(round(tokens * run / total))
+    cuts[-1] = tokens
+    return [b - a for a, b in zip(cuts, cuts[1:])]
+
+
+def _blocks(x, rows):
+    """x [..., m, k] with zeros up to whole blocks, as [..., m / rows, rows, k / 128, 128]."""
+    m, k = x.shape[-2:]
+    x = torch.nn.functional.pad(x, (0, -k % BLOCK, 0, -m % rows))
+    return x.unflatten(-1, (-1, BLOCK)).unflatten(-3, (-1, rows))
+
+
+def _quantize(x, rows):
+    """e4m3 values and exponents of the scales (a power of two for rows x 128 values) of x [..., m, k] in 32 bits: the smallest that
+    bring a block's largest value to 448 or less."""
+    b = _blocks(x.float(), rows)
+    amax = b.abs().amax(dim=(-3, -1))
+    mantissa, exponent = torch.frexp(amax)                       # 448 = 0.875 x 2^9
+    e = torch.where(mantissa <= E4M3_MAX / 512, exponent - 9, exponent - 8).clamp(-127, 127)
+    e = torch.where(amax > 0, e, torch.zeros_like(e))
+    q = torch.ldexp(b, -e[..., :, None, :, None]).flatten(-2).flatten(-3, -2)[..., : x.shape[-2], : x.shape[-1]]
+    return q.to(torch.float8_e4m3fn), e
+
+
+def _scales(e):
+    """Exponents as 8-bit scales whose rows lie a multiple of four apart, as the package keeps them."""
+    kept = torch.zeros(*e.shape[:-1], (e.shape[-1] + 3) // 4 * 4, dtype=torch.uint8, device=e.device)
+    kept[..., : e.shape[-1]] = (e + 127).to(torch.uint8)
+    return kept.view(torch.float8_e8m0fnu)[..., : e.shape[-1]]
+
+
+def _dequantized(q, scale, rows):
+    """The values in 32 bits that e4m3 values q [..., m, k] with these scales [..., m / rows, k / 128] stand for."""
+    s = scale.float().repeat_interleave(rows, -2)[..., : q.shape[-2], :].repeat_interleave(BLOCK, -1)[..., : q.shape[-1]]
+    return q.float() * s
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, std=1.0, dtype=torch.bfloat16):
+        return (torch.randn(*shape, device="cuda", generator=gen) * std).to(dtype)
+
+    kind, s = case["kind"], {"kind": case["kind"]}
+    if kind == "experts":
+        t, e, h, f = case["tokens"], case["experts"], case["hidden"], case["ffn"]
+        s["sizes"] = _group_sizes(t, e, case["skew"], seed)
+        s["ends"] = torch.tensor(s["sizes"]).cumsum(0).to(device="cuda", dtype=torch.int32)
+        s["train"] = case["train"]
+        s["x"], s["w"] = normal(t, h).requires_grad_(case["train"]), normal(e, f, h, std=h ** -0.5).requires_grad_(case["train"])
+        s["dy"] = normal(t, f, std=1e-2) if case["train"] else None
+    elif kind == "fp8":
+        m, e, k, n = case["rows"], case["experts"], case["k"], case["n"]
+        s["sizes"] = _group_sizes(m, e, case["skew"], seed) if e else None
+        s["ends"] = torch.tensor(s["sizes"]).cumsum(0).to(device="cuda", dtype=torch.int32) if e else None
+        # activations have a few channels much larger than the rest
+        s["x"] = (normal(m, k, dtype=torch.float32) * torch.exp(normal(k, std=1.0, dtype=torch.float32))).to(torch.bfloat16)
+        q, exponent = _quantize(normal(*([e] if e else []), n, k, std=k ** -0.5), BLOCK)
+        s["w"], s["w_scale"] = q, _scales(exponent)
+    else:
+        rows, vocab = case["rows"], case["vocab"]
+        width = (vocab + 63) // 64 * 64 if case["padded"] else vocab
+        s["vocab"], s["reduction"] = vocab, "mean" if case["mean"] else "sum"
+        logits = normal(rows, width, std=2.0, dtype=DTYPES[case["dtype"]])
+        s["tokens"] = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+        now = _token_logp(logits[:, :vocab].float(), s["tokens"])[0]
+        s["logits"] = logits.requires_grad_(True)
+        # the policy that sampled is some steps behind, the reference further; the baseline lags behind the rewards
+        s["old"] = now + normal(rows, std=0.2, dtype=torch.float32)
+        s["ref"] = now + normal(rows, std=0.5, dtype=torch.float32) if case["kl"] else None
+        s["advantages"] = normal(rows, dtype=torch.float32) + 0.25
+        s["weights"] = (torch.rand(rows, device="cuda", generator=gen) < 0.9).float()     # the rest is padding
+        s["weights"][0] = 1.0
+    return s
+
+
+# ---- one pass, by elementary operations -----------------------------------------------------------------------------
+def _grouped(x, w, sizes):
+    """x's groups of rows, each times its expert's weights transposed, in 32 bits."""
+    return torch.cat([a @ b.t() for a, b in zip(x.float().split(sizes), w.float())])
+
+
+def _experts(s):
+    x, w, sizes = s["x"].detach().float(), s["w"].detach().float(), s["sizes"]
+    y = _grouped(x, w, sizes).to(torch.bfloat16)
+    if not s["train"]:
+        return [y]
+    dy = s["dy"].float()
+    dx = torch.cat([g @ b for g, b in zip(dy.split(sizes), w)])
+    dw = torch.stack([g.t() @ a for g, a in zip(dy.split(sizes), x.split(sizes))])
+    return [y, dx.to(torch.bfloat16), dw.to(torch.bfloat16)]
+
+
+def _fp8(s):
+    q, exponent = _quantize(s["x"], 1)
+    x = _dequantized(q, _scales(exponent), 1)
+    w = _dequantized(s["w"], s["w_scale"], BLOCK)
+    y = x @ w.t() if s["sizes"] is None else _grouped(x, w, s["sizes"])
+    return [y.to(torch.bfloat16)]
+
+
+def _token_logp(z, tokens):
+    """log p(token), and the probabilities, of logits z [rows, vocab] in 32 bits."""
+    z = z - z.amax(1, keepdim=True)
+    p = z.exp()
+    total = p.sum(1, keepdim=True)
+    return (z.gather(1, tokens[:, None]) - total.log())[:, 0], p / total
+
+
+def _policy(s):
+    logits, tokens, vocab, a, w = s["logits"].detach(), s["tokens"], s["vocab"], s["advantages"], s["weights"]
+    logp, p = _token_logp(logits[:, :vocab].float(), tokens)
+    ratio = (logp - s["old"]).exp()
+    plain, clipped = ratio * a, ratio.clamp(1 - CLIP[0], 1 + CLIP[1]) * a
+    term, slope = -torch.minimum(plain, clipped), torch.where(plain <= clipped, -plain, torch.zeros_like(plain))
+    if s["ref"] is not None:
+        back = s["ref"] - logp
+        term, slope = term + KL * (back.exp() - back - 1), slope + KL * (1 - back.exp())
+    over = w.sum() if s["reduction"] == "mean" else torch.ones((), device=w.device)
+    loss = ((w * term).double().sum() / over).float()                    # a long sum of terms of both signs
+    slope = (slope * w / over)[:, None]
+    grad = torch.zeros_like(logits, dtype=torch.float32)
+    grad[:, :vocab] = -slope * p
+    grad.scatter_add_(1, tokens[:, None], slope)
+    return [loss, logp, grad.to(logits.dtype)]
+
+
+# ---- one pass, through the package ----------------------------------------------------------------------------------
+def _own(s):
+    if s["kind"] == "experts":
+        from mccl_b200.ops.gemm import grouped_gemm
+        y = grouped_gemm(s["x"], s["w"], s["ends"])
+        return [y.detach(), *torch.autograd.grad(y, [s["x"], s["w"]], s["dy"])] if s["train"] else [y]
+    if s["kind"] == "fp8":
+        from mccl_b200.ops.fp8 import BlockScaled, fp8_gemm
+        return [fp8_gemm(s["x"], BlockScaled(s["w"], s["w_scale"]), ends=s["ends"])]
+    from mccl_b200.ops.loss import fused_policy_loss
+    loss, logp = fused_policy_loss(s["logits"], s["tokens"], s["old"], s["advantages"], ref_logp=s["ref"], weights=s["weights"], clip=CLIP,
+                                   kl_coef=KL if s["ref"] is not None else 0.0, vocab=s["vocab"], reduction=s["reduction"])
+    return [loss.detach(), logp, *torch.autograd.grad(loss, [s["logits"]])]
+
+
+def run(s):
+    if own:
+        return _own(s)
+    return {"experts": _experts, "fp8": _fp8, "policy": _policy}[s["kind"]](s)
+
+
+# ---- what a pass cannot do without ----------------------------------------------------------------------------------
+def work(case):
+    if case["kind"] == "experts":
+        t, h, f = case["tokens"], case["hidden"], case["ffn"]
+        weights = min(case["experts"], t) * h * f
+        once = 2 * (t * h + weights + t * f)
+        return {"bytes": 2 * once if case["train"] else once, "flops": (6 if case["train"] else 2) * t * h * f}
+    if case["kind"] == "fp8":
+        m, k, n = case["rows"], case["k"], case["n"]
+        weights = (min(case["experts"], m) or 1) * n * k
+        return {"bytes": 2 * m * k + weights + weights / BLOCK ** 2 + 2 * m * n, "flops": 2 * m * n * k}
+    # the gradient needs the sums of whole rows, and takes the loss's own gradient: the logits are read in both passes
+    cells = case["rows"] * case["vocab"]
+    return {"bytes": 3 * cells * (4 if case["dtype"] == "fp32" else 2), "flops": 8 * cells}
+
+
+# ---- the definitions in 64 bits -------------------------------------------------------------------------------------
+def _rounded_e4m3(v):
+    """The nearest value of 4 exponent and 3 mantissa bits, the even one of two; |v| <= 448."""
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    return torch.round(v / step) * step
+
+
+def _exact_fp8(x):
+    m, k = x.shape
+    b = torch.nn.functional.pad(x.double(), (0, -k % BLOCK)).view(m, -1, BLOCK)
+    amax = b.abs().amax(2, keepdim=True)
+    scale = torch.where(amax > 0, torch.exp2(torch.ceil(torch.log2(amax / E4M3_MAX)).clamp(-127, 127)), torch.ones_like(amax))
+    return (_rounded_e4m3(b / scale) * scale).view(m, -1)[:, :k]
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["kind"] == "policy":
+        z, w, a = s["logits"].detach()[:, : s["vocab"]].double(), s["weights"].double(), s["advantages"].double()
+        norm = torch.logsumexp(z, 1)
+        logp = z[torch.arange(len(z), device=z.device), s["tokens"]] - norm
+        r = torch.exp(logp - s["old"].double())
+        bounded = torch.min(torch.max(r, torch.full_like(r, 1 - CLIP[0])), torch.full_like(r, 1 + CLIP[1]))
+        term, slope = torch.max(-a * r, -a * bounded), -a * r * ((-a * r) >= (-a * bounded))
+        if s["ref"] is not None:
+            d = s["ref"].double() - logp
+            term, slope = term + KL * (torch.expm1(d) - d), slope - KL * torch.expm1(d)
+        over = w.sum() if case["mean"] else 1.0
+        slope = slope * w / over
+        grad = torch.exp(z - norm[:, None]) * -slope[:, None]
+        grad[torch.arange(len(z), device=z.device), s["tokens"]] += slope
+        return [(w * term).sum() / over, logp, torch.nn.functional.pad(grad, (0, s["logits"].shape[1] - s["vocab"]))]
+    if case["kind"] == "experts":
+        x, w = s["x"].detach().double(), s["w"].detach().double()
+        dy = s["dy"].double() if case["train"] else None
+    else:
+        scale = torch.exp2(s["w_scale"].view(torch.uint8).double() - 127)
+        n, k = s["w"].shape[-2:]
+        x = _exact_fp8(s["x"])
+        w = s["w"].double() * scale[..., torch.arange(n, device="cuda") // BLOCK, :][..., torch.arange(k, device="cuda") // BLOCK]
+        dy = None
+        if s["sizes"] is None:
+            return [x @ w.t()]
+    y = torch.empty(x.shape[0], w.shape[1], dtype=torch.float64, device="cuda")
+    dx, dw, lo = torch.empty_like(x), torch.zeros_like(w), 0
+    for i, size in enumerate(s["sizes"]):
+        rows = slice(lo, lo + size)
+        y[rows] = x[rows] @ w[i].t()
+        if dy is not None:
+            dx[rows], dw[i] = dy[rows] @ w[i], dy[rows].t() @ x[rows]
+        lo += size
+    return [y] if dy is None else [y, dx, dw]
