@@ -87,10 +87,10 @@ def draw(rng):
 
 # ---- what the program has in hand -----------------------------------------------------------------------------------
 def _group_sizes(tokens, experts, skew, seed):
-    """How many rows each expert gets: shares spread by exp(skew x normal), or top-k's distinct experts for a few rows."""
+    """How many rows each expert gets: shares spread by exp(skew x normal), drawn row by row where there are few."""
     rng = random.Random(seed)
     share = [math.exp(skew * rng.gauss(0, 1)) for _ in range(experts)]
-    if tokens < 4 * experts:                                     # few rows: drawn one by one
+    if tokens < 4 * experts:
         picked = rng.choices(range(experts), share, k=tokens)
         return [picked.count(e) for e in range(experts)]
     total, run, cuts = sum(share), 0.0, [0]
@@ -161,7 +161,7 @@ def prepare(case, seed):
         s["vocab"], s["reduction"] = vocab, "mean" if case["mean"] else "sum"
         logits = normal(rows, width, std=2.0, dtype=DTYPES[case["dtype"]])
         s["tokens"] = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
-        now = _token_logp(logits[:, :vocab].float(), s["tokens"])[0]
+        now = _token_logp(logits[:, :vocab].float(), s["tokens"])[0].float()
         s["logits"] = logits.requires_grad_(True)
         # the policy that sampled is some steps behind, the reference further; the baseline lags behind the rewards
         s["old"] = now + normal(rows, std=0.2, dtype=torch.float32)
@@ -198,29 +198,29 @@ def _fp8(s):
 
 
 def _token_logp(z, tokens):
-    """log p(token), and the probabilities, of logits z [rows, vocab] in 32 bits."""
+    """log p(token), in 64 bits, and the probabilities, of logits z [rows, vocab] in 32 bits."""
     z = z - z.amax(1, keepdim=True)
     p = z.exp()
-    total = p.sum(1, keepdim=True)
-    return (z.gather(1, tokens[:, None]) - total.log())[:, 0], p / total
+    total = p.sum(1, keepdim=True, dtype=torch.float64)
+    return (z.gather(1, tokens[:, None]) - total.log())[:, 0], p / total.float()
 
 
 def _policy(s):
     logits, tokens, vocab, a, w = s["logits"].detach(), s["tokens"], s["vocab"], s["advantages"], s["weights"]
     logp, p = _token_logp(logits[:, :vocab].float(), tokens)
-    ratio = (logp - s["old"]).exp()
+    ratio = (logp - s["old"]).exp()                                      # in 64 bits: some lie next to the clamp's ends
     plain, clipped = ratio * a, ratio.clamp(1 - CLIP[0], 1 + CLIP[1]) * a
     term, slope = -torch.minimum(plain, clipped), torch.where(plain <= clipped, -plain, torch.zeros_like(plain))
     if s["ref"] is not None:
         back = s["ref"] - logp
         term, slope = term + KL * (back.exp() - back - 1), slope + KL * (1 - back.exp())
     over = w.sum() if s["reduction"] == "mean" else torch.ones((), device=w.device)
-    loss = ((w * term).double().sum() / over).float()                    # a long sum of terms of both signs
-    slope = (slope * w / over)[:, None]
+    loss = ((w * term).sum() / over).float()                             # a long sum of terms of both signs
+    slope = (slope * w / over)[:, None].float()
     grad = torch.zeros_like(logits, dtype=torch.float32)
     grad[:, :vocab] = -slope * p
     grad.scatter_add_(1, tokens[:, None], slope)
-    return [loss, logp, grad.to(logits.dtype)]
+    return [loss, logp.float(), grad.to(logits.dtype)]
 
 
 # ---- one pass, through the package ----------------------------------------------------------------------------------
