@@ -9,9 +9,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include "f32x2.cuh"
 #include "mccl.h"
 #include "mccl_ops.h"
+#include "online_softmax.cuh"
 
 namespace {
 
@@ -23,55 +23,15 @@ constexpr int kCeThreads = 256;
 constexpr int kCeUnroll = 4;                   // 16-byte pieces in flight per thread in long rows: with one, the row's loads wait for each other
 constexpr int64_t kIgnored = -100;             // the target value torch's cross-entropy leaves out
 
-struct MaxSum { float m, s; };                 // running maximum and sum of exp(x - m)
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLowest = -3.402823466e38f;    // a maximum of nothing: below every finite bf16 number, and minus itself zero
-__device__ __forceinline__ MaxSum combine(MaxSum a, MaxSum b) {
-  const float m = fmaxf(a.m, b.m);
-  return MaxSum{m, a.s * __expf(a.m - m) + b.s * __expf(b.m - m)};
-}
-__device__ __forceinline__ void unpack(const uint4& q, float* f) {
+__device__ __forceinline__ void unpack(const uint4& q, float (&f)[8]) {
   const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&q);
 #pragma unroll
   for (int k = 0; k < 4; ++k) { const float2 t = __bfloat1622float2(e[k]); f[2 * k] = t.x; f[2 * k + 1] = t.y; }
 }
-// Values enter one after another: s = s exp(m - x) + 1 where x is a new maximum and s + exp(x - m) where not.  The maximum
-// is subtracted before anything is scaled: exp(x - m) as 2^(x log2e - m log2e) would save an instruction, but it rounds
-// m log2e (an error of |m| 2^-24 in every exponent) and overflows for logits near the type's lowest value, which masks are made
-// of.
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ void add(MaxSum& a, bool up, float e) { a.s = up ? __fmaf_rn(a.s, e, 1.f) : __fadd_rn(a.s, e); }
-__device__ __forceinline__ void push(MaxSum& a, float x) {
-  add(a, x > a.m, ex2(-fabsf((x - a.m) * kLog2e)));
-  a.m = fmaxf(a.m, x);
-}
-// Eight of them.  Instructions bound the forward pass here, at eight values of nine slots each a turn (8192 x 50257: 201 us):
-// the eight maxima first, then differences and products two at a time, then the sums, predicated: 148 us, 5.6 TB/s.  (With a
-// branch for a new maximum, which some lane of a warp takes nearly always: 254 us.)
 __device__ __forceinline__ void push8(MaxSum& a, const uint4& q) {
-  float f[8], m[9], e[8];
+  float f[8];
   unpack(q, f);
-  m[0] = a.m;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) m[k + 1] = fmaxf(m[k], f[k]);
-#pragma unroll
-  for (int k = 0; k < 8; k += 2) {
-    float d0, d1;
-    split((f2(f[k], f[k + 1]) + f2(-m[k], -m[k + 1])) * f2(kLog2e), &d0, &d1);
-    e[k] = ex2(-fabsf(d0));
-    e[k + 1] = ex2(-fabsf(d1));
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) add(a, f[k] > m[k], e[k]);
-  a.m = m[8];
-}
-
-// The part of a row between its first and last 16-byte boundary: [head, head + 8 * vecs) of n elements.
-struct Span { int head, vecs; };
-__device__ __forceinline__ Span spanOf(const __nv_bfloat16* x, int n) {
-  int head = (int)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / 2;
-  if (head > n) head = n;
-  return Span{head, (n - head) / 8};
+  pushAll(a, f);
 }
 
 template <int U>

@@ -93,6 +93,58 @@ py::object crossEntropy(const Tensor& logits, const Tensor& targets, std::option
   return py::cast(CrossEntropyFn::apply(logits, targets, vocab ? *vocab : logits.size(1)));
 }
 
+// ---- policy loss ----------------------------------------------------------------------------------------------------
+struct PolicyOptions { double clipLow, clipHigh, klCoef; int64_t vocab; bool mean; };
+
+mcclDataType_t logitsType(const Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 ? mcclBfloat16 : t.scalar_type() == at::kHalf ? mcclFloat16 : mcclFloat32;
+}
+
+// Outputs: the loss and every token's log-probability (a constant).  The gradient goes to memory of its own: the logits stay as they are.
+struct PolicyLossFn : torch::autograd::Function<PolicyLossFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const Tensor& old, const Tensor& advantages,
+                               const std::optional<Tensor>& ref, const std::optional<Tensor>& weights, const PolicyOptions& o) {
+    Below below;
+    c10::cuda::CUDAGuard guard(logits.device());
+    const int64_t rows = logits.size(0);
+    auto f32 = logits.options().dtype(at::kFloat);
+    Tensor logp = at::empty({rows}, f32), stats = at::empty({3 * rows + 1}, f32), loss = at::empty({}, f32);
+    Tensor term = at::empty({rows}, f32.dtype(at::kDouble));
+    float* inverse = stats.data_ptr<float>() + 3 * rows;
+    check(mcclPolicyLossForward(logits.data_ptr(), logitsType(logits), rows, std::max(logits.stride(0), logits.size(1)), (int)o.vocab,
+                                tokens.data_ptr<int64_t>(), old.data_ptr<float>(), ref ? ref->data_ptr<float>() : nullptr, advantages.data_ptr<float>(),
+                                weights ? weights->data_ptr() : nullptr, weights && weights->scalar_type() == at::kBool, o.clipLow, o.clipHigh, o.klCoef,
+                                o.mean, logp.data_ptr<float>(), term.data_ptr<double>(), stats.data_ptr<float>(), loss.data_ptr<float>(), inverse,
+                                streamOf(logits)), "mcclPolicyLossForward");
+    counters().loss += rows > 0 ? 2 : 1;
+    ctx->save_for_backward({logits, tokens, stats});
+    ctx->saved_data["vocab"] = o.vocab;
+    ctx->mark_non_differentiable({logp});
+    return {loss, logp};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
+    Below below;
+    c10::cuda::CUDAGuard guard(logits.device());
+    const int64_t rows = logits.size(0), width = logits.size(1);
+    Tensor go = g[0].to(at::kFloat), grad = at::empty({rows, width}, logits.options());
+    check(mcclPolicyLossBackward(logits.data_ptr(), logitsType(logits), rows, std::max(logits.stride(0), width), grad.data_ptr(), width,
+                                 (int)ctx->saved_data["vocab"].toInt(), (int)width, tokens.data_ptr<int64_t>(), stats.data_ptr<float>(),
+                                 go.data_ptr<float>(), stats.data_ptr<float>() + 3 * rows, streamOf(logits)), "mcclPolicyLossBackward");
+    counters().loss += rows > 0;
+    return once({grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// (loss, logp).  The caller has checked types, shapes and devices.
+py::object policyLoss(const Tensor& logits, const Tensor& tokens, const Tensor& old, const Tensor& advantages, const std::optional<Tensor>& ref,
+                      const std::optional<Tensor>& weights, double clipLow, double clipHigh, double klCoef, int64_t vocab, bool mean) {
+  TORCH_CHECK(!recorded() && ordinary(logits), "fused_policy_loss: not under tracing, a dispatch mode or torch.func");
+  variable_list r = PolicyLossFn::apply(logits, tokens, old, advantages, ref, weights, PolicyOptions{clipLow, clipHigh, klCoef, vocab, mean});
+  return py::make_tuple(r[0], r[1]);
+}
+
 // ---- optimizer ------------------------------------------------------------------------------------------------------
 mcclStream_t pick(const Tensor& t, std::optional<int64_t> stream) {
   return stream ? reinterpret_cast<mcclStream_t>(*stream) : streamOf(t);
@@ -230,6 +282,7 @@ std::pair<Tensor, Tensor> geluBackward(const Tensor& x, const Tensor& dy) {
 void bindOps(py::module_& m) {
   m.def("layer_norm", &layerNorm);
   m.def("cross_entropy", &crossEntropy);
+  m.def("policy_loss", &policyLoss);
   m.def("adamw", &adamw);
   m.def("sum_squares", &sumSquares);
   m.def("gemm", &gemm);

@@ -123,6 +123,18 @@ mcclResult_t mcclCrossEntropyMeanBackward(void* logits, int64_t rows, int64_t ld
                                           const float* lse, const float* gradOut, const float* inverse, mcclStream_t stream);
 mcclResult_t mcclCrossEntropyBackward(void* logits, int64_t rows, int64_t ld, int vocab, int width, const int64_t* targets,
                                       const float* lse, const float* gradOut, mcclStream_t stream);
+/* Clipped policy loss with a KL term over logits [rows, ld] (bfloat16, float16 or float32; columns from vocab on take no part):
+ *   lp = z[token] - logsumexp(z), r = exp(lp - old), l = -min(r A, clamp(r, 1 - low, 1 + high) A) + kl (exp(ref - lp) - (ref - lp) - 1),
+ * *loss = sum of w l, with `mean` divided by the sum of w (zero where that is zero).  logp[row] = lp.  refLogp (nullable: no KL term);
+ * weights (nullable: ones): floats, or bytes of truth values.  term: rows doubles, stats: 3 x rows floats of work memory, the latter
+ * and *inverse kept for the backward pass, which writes grad [rows, gradLd] (zeros from vocab to width). */
+mcclResult_t mcclPolicyLossForward(const void* logits, mcclDataType_t dt, int64_t rows, int64_t ld, int vocab, const int64_t* tokens,
+                                   const float* oldLogp, const float* refLogp, const float* advantages, const void* weights, int boolWeights,
+                                   double clipLow, double clipHigh, double klCoef, int mean, float* logp, double* term, float* stats, float* loss,
+                                   float* inverse, mcclStream_t stream);
+mcclResult_t mcclPolicyLossBackward(const void* logits, mcclDataType_t dt, int64_t rows, int64_t ld, void* grad, int64_t gradLd, int vocab,
+                                    int width, const int64_t* tokens, const float* stats, const float* gradOut, const float* inverse,
+                                    mcclStream_t stream);
 /* LayerNorm over bf16 rows of D elements, D % 8 == 0 and D <= 4096.  The backward passes need partial:
  * mcclLayerNormPartials(rows) x 2 x D (3 x D for the Add form) floats of work memory. */
 int          mcclLayerNormPartials(int64_t rows);
