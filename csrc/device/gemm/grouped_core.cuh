@@ -1,0 +1,304 @@
+// Products of ragged groups of rows on the tcgen05 tensor cores: each group of rows with the weights of its expert.
+//
+//   FORWARD   y[t, n]     = sum over k of x[t, k] w[e, n, k]          e: the group of row t
+//   DATA      dx[t, k]    = sum over n of dy[t, n] w[e, n, k]
+//   WEIGHT    dw[e, n, k] = sum over the rows t of group e of dy[t, n] x[t, k]
+//
+// The groups are given by their ends on the device; the host knows only the number of rows.  Every CTA reads the ends, lays the
+// tiles of all groups end to end and takes every gridDim-th of them.  A tile is 128 rows of ONE group (or of one expert's weights)
+// by BN columns: the rows of a tile that belong to the next group are loaded and multiplied like any others and not stored, so a
+// group's last tile costs a whole one (half a tile a group on average; nothing is padded or copied).
+//
+// The operands lie in memory as the model keeps them, so some have the contracted dimension inside (K-major, one box of 64
+// elements x rows) and some outside (MN-major, boxes of 64 columns x 64 contracted rows); the matrix descriptors say which, and
+// nothing is transposed.  In WEIGHT the contracted dimension is the ragged one: the rows of the last block behind the
+// group's end are cleared in shared memory before the tensor core reads them (they may hold anything, and 0 x Inf is no zero).
+//
+//   warp 0      TMA producer
+//   warp 1      issues the MMAs (one thread); clears the rows behind a group's end
+//   warp 2      allocates and frees tensor memory
+//   warps 4-11  epilogue: four lane quarters x two halves of the columns
+// Every wait is bounded; a role that gives up records it and all roles leave.  No counterpart in the reference.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "gemm_core.cuh"
+
+namespace mccl {
+namespace grouped {
+
+using gemm::BM;
+constexpr int kThreads = 384, kEpiWarps = 8, kMaxGroups = 1024;
+constexpr int kStageK = 128;           // bytes of the contracted dimension a stage holds, one swizzled row: 64 bf16
+enum Mode { FORWARD = 0, DATA = 1, WEIGHT = 2 };
+
+struct Args {
+  CUtensorMap mapA;                    // FORWARD / DATA: x or dy [T, contracted], box 64 x 128; WEIGHT: dy [T, N], box 64 x 64
+  CUtensorMap mapB;                    // FORWARD: w [E, N, K], box 64 x BN; DATA: the same, box 64 x 64; WEIGHT: x [T, K], box 64 x 64
+  const void* ends;                    // [groups] int32 or int64
+  int ends64, groups;
+  int rows;                            // T
+  int contracted;                      // FORWARD: K, DATA: N
+  int tileRows, width;                 // WEIGHT: N (rows of an expert's output); columns of the output
+  __nv_bfloat16* out;                  // [T, width], or WEIGHT: [E, tileRows, width]
+  int* errFlag;
+  uint64_t budgetNs;
+};
+
+template <int BN> struct Smem {
+  static constexpr int A_BYTES = BM * kStageK, B_BYTES = BN * kStageK;
+  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
+  static constexpr int TABLE_BYTES = 2 * (kMaxGroups + 4) * 4;
+  static constexpr int TOTAL = TILE_BYTES + TABLE_BYTES + 256 + 1024;
+};
+
+// MN-major bf16 tile written by TMA with the 128-byte swizzle: chunks of 64 columns, each 64 contracted rows of 128 bytes.
+// Leading byte offset = distance of two chunks, stride byte offset = distance of two groups of eight contracted rows.
+__device__ __forceinline__ uint64_t smemDescMn(const void* tile) {
+  uint64_t d = 0;
+  d |= (uint64_t)((umma::smemAddr(tile) & 0x3ffff) >> 4);
+  d |= (uint64_t)(8192 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void tmaLoad3d(void* smemDst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      :: "r"(umma::smemAddr(smemDst)), "l"(map), "r"(umma::smemAddr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// The groups as every role sees them: group e holds the rows [start[e], start[e + 1]); the tiles of all groups up to e number
+// prefix[e + 1].  Ends that fall or lie outside the rows are read as the largest so far, within [0, T]: no access depends on them.
+struct Groups {
+  int* start;
+  int* prefix;
+};
+
+// One warp.  `perRowTile`: column tiles of one row tile, or WEIGHT (rowTile 0): tiles of an expert.
+__device__ __forceinline__ void readGroups(const Groups& g, const void* ends, int ends64, int groups, int T, int rowTile, int perRowTile, int lane) {
+  int last = 0, tiles = 0;
+  if (lane == 0) { g.start[0] = 0; g.prefix[0] = 0; }
+  for (int e0 = 0; e0 < groups; e0 += 32) {
+    const int e = e0 + lane;
+    int end = 0;
+    if (e < groups) {
+      const int64_t v = ends64 ? static_cast<const int64_t*>(ends)[e] : (int64_t) static_cast<const int32_t*>(ends)[e];
+      end = (int)(v < 0 ? 0 : v > T ? T : v);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, end, o); if (lane >= o && v > end) end = v; }
+    if (end < last) end = last;
+    int begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = last;
+    int n = e < groups ? (rowTile == 0 ? perRowTile : (end - begin + rowTile - 1) / rowTile * perRowTile) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += v; }
+    if (e < groups) { g.start[e + 1] = end; g.prefix[e + 1] = tiles + n; }
+    last = __shfl_sync(0xffffffffu, end, 31);
+    tiles += __shfl_sync(0xffffffffu, n, 31);
+  }
+}
+
+// Tile t of all, which is one of group e: its first row and first column.  The tiles of a group go panel by panel of eight row tiles, the row
+// fastest, so that what runs at a time shares a few weight tiles.
+struct Tile { int e, row, col; };
+__device__ __forceinline__ void tileAt(const Groups& g, int t, int e, int rowTiles, int colTiles, int rowStep, int colStep, Tile* out) {
+  const int l = t - g.prefix[e];
+  const int p = l / (8 * colTiles), within = l - p * 8 * colTiles, in = min(8, rowTiles - 8 * p);
+  out->e = e;
+  out->row = (p * 8 + within % in) * rowStep;
+  out->col = (within / in) * colStep;
+}
+
+// A wait of a whole warp: all its lanes get the same answer, so that they leave a loop together.  False where it took too long, or
+// where another role has given up.
+template <bool PARKED>
+__device__ __forceinline__ bool waitWarp(uint64_t* bar, uint32_t parity, uint64_t budget, volatile int* sFail) {
+  bool ok = *sFail == 0;
+  if (ok) ok = PARKED ? umma::mbarWaitParked(bar, parity, budget) : umma::mbarWait(bar, parity, budget);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  *sFail = 1;
+  return false;
+}
+
+template <int BN, int MODE>
+__global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_constant__ Args a) {
+  using S = Smem<BN>;
+  constexpr int ST = S::STAGES;
+  constexpr int CK = 64;                                   // contracted elements a stage
+  extern __shared__ uint8_t smemRaw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + ST * S::A_BYTES;
+  const Groups g{reinterpret_cast<int*>(smem + S::TILE_BYTES), reinterpret_cast<int*>(smem + S::TILE_BYTES) + kMaxGroups + 4};
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::TILE_BYTES + S::TABLE_BYTES);
+  uint64_t* full = bars;                                   // [ST] TMA -> MMA
+  uint64_t* empty = bars + ST;                             // [ST] MMA -> TMA
+  uint64_t* tmemFull = bars + 2 * ST;                      // [2] MMA -> epilogue
+  uint64_t* tmemEmpty = bars + 2 * ST + 2;                 // [2] epilogue -> MMA
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 4);
+  volatile int* sFail = reinterpret_cast<volatile int*>(tmemSlot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int colTiles = (a.width + BN - 1) / BN;
+  const int wRowTiles = MODE == WEIGHT ? (a.tileRows + BM - 1) / BM : 0;
+  const uint64_t budget = a.budgetNs;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) { umma::mbarInit(&full[s], 1); umma::mbarInit(&empty[s], 1); }
+    for (int i = 0; i < 2; ++i) { umma::mbarInit(&tmemFull[i], 1); umma::mbarInit(&tmemEmpty[i], kEpiWarps); }
+    *sFail = 0;
+    umma::fenceBarrierInit();
+    umma::prefetchTensorMap(&a.mapA);
+    umma::prefetchTensorMap(&a.mapB);
+  }
+  if (warp == 2) { umma::tmemAlloc(tmemSlot, gemm::kTmemCols); umma::tmemRelinquish(); }
+  if (warp == 3) readGroups(g, a.ends, a.ends64, a.groups, a.rows, MODE == WEIGHT ? 0 : BM, MODE == WEIGHT ? wRowTiles * colTiles : colTiles, lane);
+  umma::tcFenceBefore();
+  __syncthreads();
+  umma::tcFenceAfter();
+  const uint32_t tmemBase = *tmemSlot;
+  const int totalTiles = g.prefix[a.groups];
+  const int kBlocks = (a.contracted + CK - 1) / CK;        // FORWARD / DATA; WEIGHT: of the group
+  // Tile t, and how many blocks of the contracted dimension it has; `e` is carried from the tile before.
+  auto at = [&](int t, int* e, Tile* tile) -> int {
+    if constexpr (MODE == WEIGHT) {
+      *e = t / (wRowTiles * colTiles);
+      tileAt(g, t, *e, wRowTiles, colTiles, BM, BN, tile);
+      return (g.start[*e + 1] - g.start[*e] + CK - 1) / CK;
+    } else {
+      while (t >= g.prefix[*e + 1]) ++*e;
+      tileAt(g, t, *e, (g.start[*e + 1] - g.start[*e] + BM - 1) / BM, colTiles, BM, BN, tile);
+      return kBlocks;
+    }
+  };
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer
+    int stage = 0, e = 0; uint32_t phase = 0;
+    for (int t = blockIdx.x; t < totalTiles && *sFail == 0; t += gridDim.x) {
+      Tile tile;
+      const int blocks = at(t, &e, &tile);
+      const int row0 = g.start[tile.e];
+      for (int kb = 0; kb < blocks; ++kb) {
+        if (!umma::mbarWaitParked(&empty[stage], phase ^ 1, budget)) { *sFail = 1; atomicExch(a.errFlag, 31); break; }
+        umma::mbarExpectTx(&full[stage], S::A_BYTES + S::B_BYTES);
+        uint8_t *pa = sA + stage * S::A_BYTES, *pb = sB + stage * S::B_BYTES;
+        if (MODE == WEIGHT) {
+#pragma unroll
+          for (int c = 0; c < BM / 64; ++c) umma::tmaLoad2d(pa + c * 8192, &a.mapA, &full[stage], tile.row + c * 64, row0 + kb * CK);
+#pragma unroll
+          for (int c = 0; c < BN / 64; ++c) umma::tmaLoad2d(pb + c * 8192, &a.mapB, &full[stage], tile.col + c * 64, row0 + kb * CK);
+        } else {
+          umma::tmaLoad2d(pa, &a.mapA, &full[stage], kb * CK, row0 + tile.row);
+          if (MODE == FORWARD) {
+            tmaLoad3d(pb, &a.mapB, &full[stage], kb * CK, tile.col, tile.e);
+          } else {
+#pragma unroll
+            for (int c = 0; c < BN / 64; ++c) tmaLoad3d(pb + c * 8192, &a.mapB, &full[stage], tile.col + c * 64, kb * CK, tile.e);
+          }
+        }
+        if (++stage == ST) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (lane 0; the whole warp clears rows)
+    constexpr bool aMn = MODE == WEIGHT, bMn = MODE != FORWARD;
+    constexpr uint32_t idesc = umma::instrDescBf16(BM, BN) | (aMn ? 1u << 15 : 0) | (bMn ? 1u << 16 : 0);
+    constexpr int aStep = aMn ? 128 : 2, bStep = bMn ? 128 : 2;    // 16 contracted elements on, in 16-byte units
+    int stage = 0, e = 0, acc = 0; uint32_t phase = 0, accPhase = 0;
+    for (int t = blockIdx.x; t < totalTiles; t += gridDim.x) {
+      Tile tile;
+      const int blocks = at(t, &e, &tile);
+      if (blocks == 0) continue;                           // an expert without rows: the epilogue writes zeros by itself
+      const int tail = MODE == WEIGHT ? (g.start[tile.e + 1] - g.start[tile.e]) % CK : 0;
+      if (!waitWarp<false>(&tmemEmpty[acc], accPhase ^ 1, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 32); break; }
+      umma::tcFenceAfter();
+      const uint32_t d = tmemBase + (uint32_t)acc * 256u;
+      bool ok = true;
+      for (int kb = 0; kb < blocks; ++kb) {
+        if (!waitWarp<false>(&full[stage], phase, budget, sFail)) { ok = false; if (lane == 0) atomicExch(a.errFlag, 33); break; }
+        uint8_t *pa = sA + stage * S::A_BYTES, *pb = sB + stage * S::B_BYTES;
+        if (MODE == WEIGHT && tail != 0 && kb == blocks - 1) {
+          // Rows [tail, 64) of every chunk: whole 128-byte lines, which the swizzle does not mix.
+          for (int i = lane; i < (CK - tail) * 8; i += 32) {
+            const int off = tail * 128 + i * 16;
+#pragma unroll
+            for (int c = 0; c < BM / 64; ++c) *reinterpret_cast<uint4*>(pa + c * 8192 + off) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < BN / 64; ++c) *reinterpret_cast<uint4*>(pb + c * 8192 + off) = make_uint4(0, 0, 0, 0);
+          }
+          umma::fenceProxyAsyncShared();
+        }
+        __syncwarp();
+        umma::tcFenceAfter();
+        if (lane == 0) {
+          const uint64_t da = aMn ? smemDescMn(pa) : umma::smemDescSw128(pa), db = bMn ? smemDescMn(pb) : umma::smemDescSw128(pb);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma::mmaBf16(d, da + (uint64_t)(k * aStep), db + (uint64_t)(k * bStep), idesc, (kb | k) != 0);
+          umma::mmaCommit(&empty[stage]);
+        }
+        if (++stage == ST) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) break;
+      if (lane == 0) umma::mmaCommit(&tmemFull[acc]);
+      acc ^= 1; if (acc == 0) accPhase ^= 1;
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue
+    const int q = warp & 3, half = (warp - 4) >> 2;        // warp % 4: the TMEM lane quarter this warp may read
+    constexpr int COLS = BN / 2;
+    int e = 0, acc = 0; uint32_t accPhase = 0;
+    for (int t = blockIdx.x; t < totalTiles; t += gridDim.x) {
+      Tile tile;
+      const int blocks = at(t, &e, &tile);
+      uint32_t v[COLS];
+      if (MODE == WEIGHT && blocks == 0) {
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) v[i] = 0;
+      } else {
+        if (!waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 34); break; }
+        umma::tcFenceAfter();
+        const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * 256u + (uint32_t)(half * COLS);
+#pragma unroll
+        for (int c = 0; c < COLS / 32; ++c) umma::tmemLoad32x32(from + c * 32u, v + c * 32);
+        umma::tmemLoadWait();
+        umma::tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
+        acc ^= 1; if (acc == 0) accPhase ^= 1;
+      }
+      const int r = tile.row + q * 32 + lane, col0 = tile.col + half * COLS;
+      const int limit = MODE == WEIGHT ? a.tileRows : g.start[tile.e + 1] - g.start[tile.e];
+      if (r < limit) {
+        const size_t row = MODE == WEIGHT ? (size_t)tile.e * a.tileRows + r : (size_t)(g.start[tile.e] + r);
+        __nv_bfloat16* dst = a.out + row * (size_t)a.width + col0;
+#pragma unroll
+        for (int j = 0; j < COLS / 8; ++j) {
+          if (col0 + j * 8 >= a.width) break;
+          uint4 o;
+          __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o2[i] = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+          reinterpret_cast<uint4*>(dst)[j] = o;
+        }
+      }
+    }
+    if (MODE != WEIGHT) {                                  // rows behind the last group belong to nobody
+      const int64_t lo = (int64_t)g.start[a.groups] * a.width / 8, hi = (int64_t)a.rows * a.width / 8;
+      for (int64_t i = lo + (int64_t)blockIdx.x * (kEpiWarps * 32) + (threadIdx.x - 128); i < hi; i += (int64_t)gridDim.x * (kEpiWarps * 32))
+        reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  umma::tcFenceBefore();
+  __syncthreads();
+  if (warp == 2) umma::tmemDealloc(tmemBase, gemm::kTmemCols);
+}
+
+}  // namespace grouped
+}  // namespace mccl

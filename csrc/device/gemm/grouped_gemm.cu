@@ -1,0 +1,146 @@
+// Host side of the products of ragged groups of rows (grouped_core.cuh): tensor maps, choice of the tile, launch.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <string.h>
+
+#include <atomic>
+
+#include "../../core/core.h"
+#include "gemm_host.h"
+#include "grouped_core.cuh"
+#include "mccl_ops.h"
+
+using namespace mccl;
+using namespace mccl::grouped;
+
+namespace {
+
+// bf16 [outer][rows][cols], rows `ld` elements apart, the outer index rows * ld apart (rank 2: outer = 0); box = boxCols x boxRows,
+// 128 bytes inside.  Elements outside read as zero.
+mcclResult_t mapOf(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxCols, uint32_t boxRows) {
+  static gemm::EncodeTiledFn fn = gemm::encodeTiled();
+  if (fn == nullptr) MCCLFAIL(mcclSystemError);
+  const cuuint64_t dims[3] = {cols, rows, outer};
+  const cuuint64_t strides[2] = {ld * 2, rows * ld * 2};
+  const cuuint32_t box[3] = {boxCols, boxRows, 1}, elemStrides[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, outer ? 3 : 2, const_cast<void*>(base), dims, strides, box, elemStrides,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    MCCL_WARN("cuTensorMapEncodeTiled failed with %d (base %p, %llu x %llu x %llu, row pitch %llu)", (int)r, base, (unsigned long long)outer,
+              (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)ld);
+    return mcclInvalidArgument;
+  }
+  return mcclSuccess;
+}
+
+// The current device, its context bound to this thread: the driver's encoder needs it, and a thread of the autograd engine that has
+// launched nothing yet has none.
+int boundDevice() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaSetDevice(dev);
+  return dev;
+}
+
+template <int BN, int MODE>
+mcclResult_t launchAs(const Args& a, int dev, int grid, cudaStream_t s) {
+  auto* kernel = groupedKernel<BN, MODE>;
+  static std::atomic<uint64_t> prepared{0};                // a bit per device: the attribute stays with the function
+  if (!(prepared.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BN>::TOTAL) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
+    prepared.fetch_or(1ull << (dev & 63));
+  }
+  kernel<<<grid, kThreads, Smem<BN>::TOTAL, s>>>(a);
+  return cudaGetLastError() == cudaSuccess ? mcclSuccess : mcclSystemError;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+struct Shape { const void* ends; int ends64, E; int64_t T; int N, K; };
+
+bool valid(const Shape& s) {
+  return s.ends != nullptr && s.E > 0 && s.E <= kMaxGroups && s.T >= 0 && s.T <= INT32_MAX - 256 && s.N > 0 && s.K > 0 && s.N % 8 == 0 && s.K % 8 == 0;
+}
+bool validRows(const void* p, int64_t ld, int cols) { return p != nullptr && aligned16(p) && ld >= cols && ld % 8 == 0; }
+
+// Columns of a tile: 256 where that gives every SM a tile, else 128 (an MMA of 128 rows takes nearly as long with 128 columns as
+// with 256, so the narrow tile is worth its while only where SMs would stand idle).
+int pickColumns(int64_t rowTiles, int width, int sms) { return width > 128 && rowTiles * ((width + 255) / 256) >= sms ? 256 : 128; }
+
+template <int MODE>
+mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn) {
+  a.errFlag = gemm::gemmErrFlag(dev);
+  if (a.errFlag == nullptr) return mcclSystemError;
+  a.budgetNs = 2000000000ull;
+  a.ends = s.ends; a.ends64 = s.ends64; a.groups = s.E; a.rows = (int)s.T;
+  const int64_t tiles = rowTiles * ((a.width + bn - 1) / bn);
+  if (tiles > INT32_MAX) return mcclInvalidArgument;
+  const int sms = gemm::gemmSmCount(), grid = (int)(tiles < sms ? tiles : sms);
+  return bn == 256 ? launchAs<256, MODE>(a, dev, grid, stream) : launchAs<128, MODE>(a, dev, grid, stream);
+}
+
+// Row tiles of all groups: at most one beside the full ones for each group.
+int64_t rowTilesAtMost(const Shape& s) { return s.T / BM + (s.T < s.E ? s.T : s.E); }
+
+}  // namespace
+
+extern "C" {
+
+int mcclGroupedGemmMaxGroups(void) { return kMaxGroups; }
+
+mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K,
+                             mcclStream_t stream) {
+  const Shape s{ends, ends64, groups, rows, N, K};
+  if (!valid(s)) return mcclInvalidArgument;
+  if (rows == 0) return mcclSuccess;
+  if (!validRows(x, ldx, K) || w == nullptr || y == nullptr || !aligned16(w) || !aligned16(y)) return mcclInvalidArgument;
+  Args a;
+  memset(&a, 0, sizeof(a));
+  const int dev = boundDevice();
+  const int64_t rt = rowTilesAtMost(s);
+  const int bn = pickColumns(rt, N, gemm::gemmSmCount());
+  MCCLCHECK(mapOf(&a.mapA, x, 0, rows, K, ldx, 64, BM));
+  MCCLCHECK(mapOf(&a.mapB, w, groups, N, K, K, 64, bn));
+  a.contracted = K; a.width = N;
+  a.out = static_cast<__nv_bfloat16*>(y);
+  return run<FORWARD>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
+}
+
+mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const void* w, void* dx, const void* ends, int ends64, int groups, int64_t rows,
+                                         int N, int K, mcclStream_t stream) {
+  const Shape s{ends, ends64, groups, rows, N, K};
+  if (!valid(s)) return mcclInvalidArgument;
+  if (rows == 0) return mcclSuccess;
+  if (!validRows(dy, lddy, N) || w == nullptr || dx == nullptr || !aligned16(w) || !aligned16(dx)) return mcclInvalidArgument;
+  Args a;
+  memset(&a, 0, sizeof(a));
+  const int dev = boundDevice();
+  const int64_t rt = rowTilesAtMost(s);
+  const int bn = pickColumns(rt, K, gemm::gemmSmCount());
+  MCCLCHECK(mapOf(&a.mapA, dy, 0, rows, N, lddy, 64, BM));
+  MCCLCHECK(mapOf(&a.mapB, w, groups, N, K, K, 64, 64));
+  a.contracted = N; a.width = K;
+  a.out = static_cast<__nv_bfloat16*>(dx);
+  return run<DATA>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
+}
+
+mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dw, const void* ends, int ends64, int groups,
+                                           int64_t rows, int N, int K, mcclStream_t stream) {
+  const Shape s{ends, ends64, groups, rows, N, K};
+  if (!valid(s) || dw == nullptr || !aligned16(dw)) return mcclInvalidArgument;
+  if (rows == 0)
+    return cudaMemsetAsync(dw, 0, (size_t)groups * N * K * 2, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? mcclSuccess : mcclSystemError;
+  if (!validRows(dy, lddy, N) || !validRows(x, ldx, K)) return mcclInvalidArgument;
+  Args a;
+  memset(&a, 0, sizeof(a));
+  const int dev = boundDevice();
+  const int64_t rt = (int64_t)groups * ((N + BM - 1) / BM);
+  const int bn = pickColumns(rt, K, gemm::gemmSmCount());
+  MCCLCHECK(mapOf(&a.mapA, dy, 0, rows, N, lddy, 64, 64));
+  MCCLCHECK(mapOf(&a.mapB, x, 0, rows, K, ldx, 64, 64));
+  a.tileRows = N; a.width = K;
+  a.out = static_cast<__nv_bfloat16*>(dw);
+  return run<WEIGHT>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
+}
+
+}  // extern "C"

@@ -7,19 +7,14 @@
 #include "../../comm/comm.h"
 #include "../../transport/cuda_mem.h"
 #include "gemm_core.cuh"
+#include "gemm_host.h"
 #include "mccl_ops.h"
 #include "gemm_core2.cuh"
 
 using namespace mccl;
 using namespace mccl::gemm;
 
-namespace {
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encodeTiled() {
+mccl::gemm::EncodeTiledFn mccl::gemm::encodeTiled() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -30,6 +25,8 @@ EncodeTiledFn encodeTiled() {
   });
   return fn;
 }
+
+namespace {
 
 // Row-major [rows, cols] bf16 matrix, box = 64 columns (128 bytes, the swizzle width) x boxRows rows.
 mcclResult_t makeMap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t boxRows) {
@@ -354,6 +351,9 @@ mcclResult_t twoSmGemm(const void* A, const void* B, void* C, void* pre, int M, 
 }
 
 }  // namespace
+
+int* mccl::gemm::gemmErrFlag(int device) { return errFlagFor(device).dev; }
+int mccl::gemm::gemmSmCount() { return smCount(); }
 
 extern "C" {
 

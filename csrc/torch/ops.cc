@@ -200,6 +200,64 @@ py::object gemm(const Tensor& x, const Tensor& w, const std::optional<Tensor>& o
   return py::cast(y);
 }
 
+// ---- products of ragged groups of rows ----------------------------------------------------------------------------------
+// Rows as the kernels take them: adjacent elements, 16-byte aligned rows.
+Tensor alignedRows(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  if (t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % per == 0)) && aligned16(t)) return t;
+  Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone();
+}
+int64_t pitchOf(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+Tensor whole(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone();
+}
+
+struct GroupedFn : torch::autograd::Function<GroupedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& xIn, const Tensor& wIn, const Tensor& ends) {
+    Below below;
+    c10::cuda::CUDAGuard guard(xIn.device());
+    Tensor x = alignedRows(xIn), w = whole(wIn);
+    const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1);
+    Tensor y = at::empty({T, N}, x.options());
+    check(mcclGroupedGemm(x.data_ptr(), pitchOf(x), w.data_ptr(), y.data_ptr(), ends.data_ptr(), ends.scalar_type() == at::kLong, (int)E, T, (int)N, (int)K,
+                          streamOf(x)), "mcclGroupedGemm");
+    counters().gemm += T > 0;
+    ctx->save_for_backward({x, w, ends});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    auto v = ctx->get_saved_variables();
+    const Tensor &x = v[0], &w = v[1], &ends = v[2];
+    Below below;
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1);
+    Tensor dy = alignedRows(g[0]);
+    const bool wide = ends.scalar_type() == at::kLong;
+    variable_list ret(3);
+    if (ctx->needs_input_grad(0)) {
+      ret[0] = at::empty({T, K}, x.options());
+      check(mcclGroupedGemmBackwardData(dy.data_ptr(), pitchOf(dy), w.data_ptr(), ret[0].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N, (int)K,
+                                        streamOf(x)), "mcclGroupedGemmBackwardData");
+      counters().gemm += T > 0;
+    }
+    if (ctx->needs_input_grad(1)) {
+      ret[1] = at::empty({E, N, K}, w.options());
+      check(mcclGroupedGemmBackwardWeight(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), ret[1].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N,
+                                          (int)K, streamOf(x)), "mcclGroupedGemmBackwardWeight");
+      counters().gemm += T > 0;
+    }
+    return once(std::move(ret));
+  }
+};
+
+// The caller has checked types, shapes and devices.
+Tensor groupedGemm(const Tensor& x, const Tensor& w, const Tensor& ends) {
+  TORCH_CHECK(!recorded() && ordinary(x) && ordinary(w) && ordinary(ends), "grouped_gemm: not under tracing, a dispatch mode or torch.func");
+  return GroupedFn::apply(x, w, ends);
+}
+
 // ---- SiLU MLP on one rank ---------------------------------------------------------------------------------------------
 // y = silu(x w_up^T) w_down^T.  The up product stores its sums beside the activation, so the backward pass is four products
 // and one elementwise pass; without gradients they are not kept.
@@ -286,6 +344,7 @@ void bindOps(py::module_& m) {
   m.def("adamw", &adamw);
   m.def("sum_squares", &sumSquares);
   m.def("gemm", &gemm);
+  m.def("grouped_gemm", &groupedGemm);
   m.def("mlp", &mlp);
   m.def("silu_both", &siluBoth);
   m.def("gelu_forward", &geluForward);

@@ -26,6 +26,19 @@ mcclResult_t mcclTpGemmKeepPre(const void* A, const void* B, void* C, void* pre,
 /* Error code the last GEMM kernel on the current device recorded (0 = none); reading clears it. */
 int mcclTpGemmLastError(void);
 
+/* ---- products of ragged groups of rows (bf16): rows [ends[e-1], ends[e]) of x [rows, K] with w[e] of w [groups, N, K] -------- */
+/* y[t] = x[t] w[e]^T; dx[t] = dy[t] w[e]; dw[e] = sum over the group of dy[t]^T x[t].  ends: on the device, int32 or (ends64) int64,
+ * read as the largest so far within [0, rows]; rows behind the last end are zero in y and dx and no part of dw.  N and K multiples of 8,
+ * pointers 16-byte aligned, x and dy with rows ld elements apart (a multiple of 8), the rest contiguous; at most
+ * mcclGroupedGemmMaxGroups() groups. */
+int          mcclGroupedGemmMaxGroups(void);
+mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y, const void* ends, int ends64, int groups, int64_t rows, int N,
+                             int K, mcclStream_t stream);
+mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const void* w, void* dx, const void* ends, int ends64, int groups,
+                                         int64_t rows, int N, int K, mcclStream_t stream);
+mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dw, const void* ends, int ends64,
+                                           int groups, int64_t rows, int N, int K, mcclStream_t stream);
+
 /* Fused all-gather -> GEMM -> activation.  xShard [M/n, K] in symmetric memory, xFull [M, K] local workspace,
  * W [N, K] local weight shard, out [M, N], flags >= 16 uint64 of device memory.  Collective over comm. */
 mcclResult_t mcclTpAllGatherGemm(mcclComm_t comm, const void* xShard, void* xFull, const void* W, void* out, void* flags,
