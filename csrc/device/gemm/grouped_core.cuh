@@ -82,6 +82,10 @@ struct Groups {
 __device__ __forceinline__ void readGroups(const Groups& g, const void* ends, int ends64, int groups, int T, int rowTile, int perRowTile, int lane) {
   int last = 0, tiles = 0;
   if (lane == 0) { g.start[0] = 0; g.prefix[0] = 0; }
+  if (ends == nullptr) {                                   // one group of all rows
+    if (lane == 0) { g.start[1] = T; g.prefix[1] = (T + rowTile - 1) / rowTile * perRowTile; }
+    return;
+  }
   for (int e0 = 0; e0 < groups; e0 += 32) {
     const int e = e0 + lane;
     int end = 0;
@@ -123,6 +127,26 @@ __device__ __forceinline__ bool waitWarp(uint64_t* bar, uint32_t parity, uint64_
   if (__all_sync(0xffffffffu, ok)) return true;
   *sFail = 1;
   return false;
+}
+
+// COLS sums of one row, as bf16, to the columns from col0 on of a row of `width`.
+template <int COLS>
+__device__ __forceinline__ void storeColumns(const uint32_t* v, __nv_bfloat16* row, int col0, int width) {
+#pragma unroll
+  for (int j = 0; j < COLS / 8; ++j) {
+    if (col0 + j * 8 >= width) break;
+    uint4 o;
+    __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o2[i] = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+    *reinterpret_cast<uint4*>(row + col0 + j * 8) = o;
+  }
+}
+// The epilogue warps' share of the rows behind the last group, which belong to nobody.
+__device__ __forceinline__ void clearRows(__nv_bfloat16* out, int from, int to, int width) {
+  const int64_t lo = (int64_t)from * width / 8, hi = (int64_t)to * width / 8;
+  for (int64_t i = lo + (int64_t)blockIdx.x * (kEpiWarps * 32) + (threadIdx.x - 128); i < hi; i += (int64_t)gridDim.x * (kEpiWarps * 32))
+    reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
 }
 
 template <int BN, int MODE>
@@ -272,27 +296,12 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
         if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
         acc ^= 1; if (acc == 0) accPhase ^= 1;
       }
-      const int r = tile.row + q * 32 + lane, col0 = tile.col + half * COLS;
+      const int r = tile.row + q * 32 + lane;
       const int limit = MODE == WEIGHT ? a.tileRows : g.start[tile.e + 1] - g.start[tile.e];
-      if (r < limit) {
-        const size_t row = MODE == WEIGHT ? (size_t)tile.e * a.tileRows + r : (size_t)(g.start[tile.e] + r);
-        __nv_bfloat16* dst = a.out + row * (size_t)a.width + col0;
-#pragma unroll
-        for (int j = 0; j < COLS / 8; ++j) {
-          if (col0 + j * 8 >= a.width) break;
-          uint4 o;
-          __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o2[i] = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
-          reinterpret_cast<uint4*>(dst)[j] = o;
-        }
-      }
+      const size_t row = MODE == WEIGHT ? (size_t)tile.e * a.tileRows + r : (size_t)g.start[tile.e] + r;
+      if (r < limit) storeColumns<COLS>(v, a.out + row * (size_t)a.width, tile.col + half * COLS, a.width);
     }
-    if (MODE != WEIGHT) {                                  // rows behind the last group belong to nobody
-      const int64_t lo = (int64_t)g.start[a.groups] * a.width / 8, hi = (int64_t)a.rows * a.width / 8;
-      for (int64_t i = lo + (int64_t)blockIdx.x * (kEpiWarps * 32) + (threadIdx.x - 128); i < hi; i += (int64_t)gridDim.x * (kEpiWarps * 32))
-        reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
-    }
+    if (MODE != WEIGHT) clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }
 
   umma::tcFenceBefore();

@@ -1,0 +1,131 @@
+// bf16 -> 8-bit floating point (e4m3) with a power-of-two scale (e8m0) for each block of 128 of a row, or of 128 rows x 128.
+//   scale = 2^e with the smallest e for which the block's largest magnitude is at most 448 2^e (a block of zeros: 1),
+//   q = the nearest e4m3 number to x / scale, the even one of two.
+// The exponent comes from the bits of the largest magnitude: 448 = 1.75 x 2^8, so it is that of the magnitude less eight, or less seven
+// where its mantissa is above 1.75.  x / scale is exact.  Numbers that are not finite take no part in the scale and become NaN.
+// Bound by memory: two bytes read, one written for each value.  No counterpart in the reference.
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "mccl.h"
+#include "mccl_ops.h"
+
+namespace {
+
+constexpr int kBlock = 128, kThreads = 256;
+
+// Magnitudes of eight bf16 numbers as one 16-bit maximum; numbers that are not finite count as zero.
+__device__ __forceinline__ uint32_t largest(const uint4& q) {
+  auto two = [](uint32_t w) {
+    w &= 0x7fff7fffu;
+    const uint32_t big = __vcmpgtu2(w, 0x7f7f7f7fu);       // all ones where not finite
+    return w & ~big;
+  };
+  const uint32_t m = __vmaxu2(__vmaxu2(two(q.x), two(q.y)), __vmaxu2(two(q.z), two(q.w)));
+  return max(m & 0xffffu, m >> 16);
+}
+// The scale's byte (its exponent plus 127) for a largest magnitude of these bf16 bits.
+__device__ __forceinline__ uint32_t scaleByte(uint32_t a) {
+  if (a == 0) return 127;
+  const int e = (int)(a >> 7) - ((a & 0x7f) <= 0x60 ? 8 : 7);
+  return (uint32_t)max(e, 0);
+}
+__device__ __forceinline__ uint32_t four(uint32_t lo, uint32_t hi, float inv) {
+  float f[4] = {__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __fmaf_rn(f[i], 0.f, f[i] * inv);          // Inf x 0: NaN, where the conversion would give 448
+  const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+  return a | b << 16;
+}
+__device__ __forceinline__ uint2 quantize(const uint4& q, uint32_t byte) {
+  const float inv = __uint_as_float((254u - byte) << 23);  // byte <= 247
+  return make_uint2(four(q.x, q.y, inv), four(q.z, q.w, inv));
+}
+
+// Sixteen threads a block of 128; the threads of a grid walk the blocks of all rows.
+__global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, uint8_t* scale, int64_t lds, int64_t rows, int K,
+                                                               int blocks) {
+  const int64_t b = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4, total = rows * blocks;
+  const int in = (threadIdx.x & 15) * 8;
+  const int64_t row = b < total ? b / blocks : 0;
+  const int blk = (int)(b - row * blocks), col = blk * kBlock + in;
+  const bool live = b < total && col < K;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (live) v = *reinterpret_cast<const uint4*>(x + row * ldx + col);
+  uint32_t a = largest(v);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const uint32_t byte = scaleByte(a);
+  if (live) *reinterpret_cast<uint2*>(q + row * K + col) = quantize(v, byte);
+  if (b < total && in == 0) scale[row * lds + blk] = (uint8_t)byte;
+}
+
+// One CTA a block of 128 x 128: each thread eight rows' pieces of eight values.
+__global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloat16* x, uint8_t* q, uint8_t* scale, int64_t lds, int rows, int K, int rowBlocks) {
+  __shared__ uint32_t warpMax[kThreads / 32];
+  const int rb = (int)(blockIdx.y % rowBlocks);
+  const int64_t outer = blockIdx.y / rowBlocks;
+  const int col = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+  x += outer * rows * K;
+  q += outer * rows * K;
+  uint4 v[8];
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = rb * kBlock + i * 16 + (threadIdx.x >> 4);
+    v[i] = r < rows && col < K ? *reinterpret_cast<const uint4*>(x + (int64_t)r * K + col) : make_uint4(0, 0, 0, 0);
+    a = max(a, largest(v[i]));
+  }
+  a = __reduce_max_sync(0xffffffffu, a);
+  if ((threadIdx.x & 31) == 0) warpMax[threadIdx.x >> 5] = a;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) a = max(a, warpMax[w]);
+  const uint32_t byte = scaleByte(a);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = rb * kBlock + i * 16 + (threadIdx.x >> 4);
+    if (r < rows && col < K) *reinterpret_cast<uint2*>(q + (int64_t)r * K + col) = quantize(v[i], byte);
+  }
+  if (threadIdx.x == 0) scale[(outer * rowBlocks + rb) * lds + blockIdx.x] = (uint8_t)byte;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+mcclResult_t launchedOk() { return cudaGetLastError() == cudaSuccess ? mcclSuccess : mcclSystemError; }
+
+}  // namespace
+
+extern "C" {
+
+mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, void* scale, int64_t ldScale, int64_t rows, int K, mcclStream_t stream) {
+  const int blocks = (K + kBlock - 1) / kBlock;
+  if (rows < 0 || K <= 0 || K > INT32_MAX - 256 || K % 16 || ldx < K || ldx % 8 || ldScale < blocks) return mcclInvalidArgument;
+  if (rows == 0) return mcclSuccess;
+  if (!x || !q || !scale || !aligned16(x) || !aligned16(q) || rows * blocks > (int64_t)INT32_MAX * 16) return mcclInvalidArgument;
+  const int64_t ctas = (rows * blocks + kThreads / 16 - 1) / (kThreads / 16);
+  quantizeRowsKernel<<<(unsigned)ctas, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q),
+                                                                                              static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
+  return launchedOk();
+}
+
+mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, void* scale, int64_t ldScale, int64_t outer, int rows, int K, mcclStream_t stream) {
+  if (outer < 0 || rows <= 0 || K <= 0 || K > INT32_MAX - 256 || rows > INT32_MAX - 256 || K % 16 || ldScale < (K + kBlock - 1) / kBlock) return mcclInvalidArgument;
+  if (outer == 0) return mcclSuccess;
+  const int rowBlocks = (rows + kBlock - 1) / kBlock;
+  if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return mcclInvalidArgument;
+  // the grid's second dimension ends at 65535: matrices in turn
+  const int64_t per = rowBlocks <= 65535 ? 65535 / rowBlocks : 0;
+  if (per == 0) return mcclInvalidArgument;
+  for (int64_t o = 0; o < outer; o += per) {
+    const int64_t n = outer - o < per ? outer - o : per;
+    quantizeTilesKernel<<<dim3((unsigned)((K + kBlock - 1) / kBlock), (unsigned)(n * rowBlocks)), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+        static_cast<const __nv_bfloat16*>(x) + o * rows * K, static_cast<uint8_t*>(q) + o * rows * K, static_cast<uint8_t*>(scale) + o * rowBlocks * ldScale,
+        ldScale, rows, K, rowBlocks);
+  }
+  return launchedOk();
+}
+
+}  // extern "C"

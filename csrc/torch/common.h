@@ -60,6 +60,20 @@ struct Below {
   c10::impl::ExcludeDispatchKeyGuard noCast{c10::autocast_dispatch_keyset};
 };
 
+// Rows of a matrix as the products' kernels take them: adjacent elements, rows at 16-byte boundaries `pitchOf` elements apart; and a
+// tensor without gaps from a 16-byte boundary on.  Copies only where they have to.
+inline Tensor alignedRows(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  if (t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % per == 0)) && aligned16(t)) return t;
+  Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone();
+}
+inline int64_t pitchOf(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+inline Tensor whole(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone();
+}
+
 // Gradients that have no graph of their own: differentiating them (backward(create_graph=True)) raises instead of counting
 // them as constants.
 inline variable_list once(variable_list&& grads) {
@@ -72,6 +86,7 @@ inline variable_list once(variable_list&& grads) {
 // One module's functions each, defined in the files of the same names.
 void bindOps(pybind11::module_& m);
 void bindComm(pybind11::module_& m);
+void bindFp8(pybind11::module_& m);
 void bindMoe(pybind11::module_& m);
 void bindGpt2(pybind11::module_& m);
 void bindLlama(pybind11::module_& m);

@@ -1,0 +1,79 @@
+// 8-bit products of the torch binding: quantisation by blocks of 128 and the block-scaled product.
+#include "common.h"
+
+namespace mccl_torch {
+namespace {
+
+constexpr int64_t kBlock = 128;
+
+int64_t blocksOf(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+// Scales as bytes, a row's blocks adjacent and rows a multiple of four bytes apart.
+Tensor scaleStore(at::IntArrayRef sizes, const Tensor& like) {
+  std::vector<int64_t> padded(sizes.begin(), sizes.end());
+  padded.back() = (padded.back() + 3) / 4 * 4;
+  return at::empty(padded, like.options().dtype(at::kByte)).narrow(-1, 0, sizes.back());
+}
+Tensor scaleRows(const Tensor& s) {
+  Tensor b = s.view(at::kByte);
+  const int64_t d = b.dim(), pitch = b.stride(d - 2);
+  const bool fits = b.stride(d - 1) == 1 && pitch >= b.size(d - 1) && pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(b.data_ptr()) & 3u) == 0 &&
+                    (d < 3 || b.stride(0) == pitch * b.size(1));
+  if (fits) return b;
+  return scaleStore(b.sizes(), b).copy_(b);
+}
+
+struct Quantized { Tensor data, scale; };       // scale: bytes
+
+Quantized quantizeRows(const Tensor& xIn) {
+  Tensor x = alignedRows(xIn);
+  const int64_t M = x.size(0), K = x.size(1);
+  Quantized r{at::empty({M, K}, x.options().dtype(at::kFloat8_e4m3fn)), scaleStore({M, blocksOf(K)}, x)};
+  check(mcclFp8QuantizeRows(x.data_ptr(), pitchOf(x), r.data.data_ptr(), r.scale.data_ptr(), r.scale.stride(0), M, (int)K, streamOf(x)), "mcclFp8QuantizeRows");
+  counters().gemm += M > 0;
+  return r;
+}
+
+// e4m3 values and e8m0 scales of bf16 x: [M, K] by blocks of 128 of a row, or (tiles) [.., N, K] by 128 x 128.
+std::pair<Tensor, Tensor> fp8Quantize(const Tensor& xIn, bool tiles) {
+  TORCH_CHECK(!recorded() && ordinary(xIn), "fp8_quantize: not under tracing, a dispatch mode or torch.func");
+  Below below;
+  c10::cuda::CUDAGuard guard(xIn.device());
+  if (!tiles) {
+    Quantized r = quantizeRows(xIn);
+    return {r.data, r.scale.view(at::kFloat8_e8m0fnu)};
+  }
+  Tensor x = whole(xIn);
+  const int64_t K = x.size(-1), N = x.size(-2), outer = x.dim() == 3 ? x.size(0) : 1;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes[sizes.size() - 2] = blocksOf(N);
+  sizes.back() = blocksOf(K);
+  Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), s = scaleStore(sizes, x);
+  check(mcclFp8QuantizeTiles(x.data_ptr(), q.data_ptr(), s.data_ptr(), s.stride(-2), outer, (int)N, (int)K, streamOf(x)), "mcclFp8QuantizeTiles");
+  counters().gemm++;
+  return {q, s.view(at::kFloat8_e8m0fnu)};
+}
+
+// x: bf16, quantised here, or e4m3 with its scales.  The caller has checked types, shapes and devices.
+Tensor fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const Tensor& wIn, const Tensor& wScale, const std::optional<Tensor>& ends) {
+  TORCH_CHECK(!recorded() && ordinary(x) && ordinary(wIn), "fp8_gemm: not under tracing, a dispatch mode or torch.func");
+  Below below;
+  c10::cuda::CUDAGuard guard(x.device());
+  Quantized a = xScale ? Quantized{alignedRows(x), scaleRows(*xScale)} : quantizeRows(x);
+  Tensor w = whole(wIn), ws = scaleRows(wScale);
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(-2), E = w.dim() == 3 ? w.size(0) : 1;
+  Tensor y = at::empty({M, N}, x.options().dtype(at::kBFloat16));
+  check(mcclFp8Gemm(a.data.data_ptr(), pitchOf(a.data), a.scale.data_ptr(), a.scale.stride(0), w.data_ptr(), ws.data_ptr(), ws.stride(-2), y.data_ptr(),
+                    ends ? ends->data_ptr() : nullptr, ends && ends->scalar_type() == at::kLong, (int)E, M, (int)N, (int)K, streamOf(x)), "mcclFp8Gemm");
+  counters().gemm += M > 0;
+  return y;
+}
+
+}  // namespace
+
+void bindFp8(py::module_& m) {
+  m.def("fp8_quantize", &fp8Quantize);
+  m.def("fp8_gemm", &fp8Gemm);
+}
+
+}  // namespace mccl_torch

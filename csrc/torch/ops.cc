@@ -201,19 +201,6 @@ py::object gemm(const Tensor& x, const Tensor& w, const std::optional<Tensor>& o
 }
 
 // ---- products of ragged groups of rows ----------------------------------------------------------------------------------
-// Rows as the kernels take them: adjacent elements, 16-byte aligned rows.
-Tensor alignedRows(const Tensor& t) {
-  const int64_t per = 16 / t.element_size();
-  if (t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % per == 0)) && aligned16(t)) return t;
-  Tensor c = t.contiguous();
-  return aligned16(c) ? c : c.clone();
-}
-int64_t pitchOf(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
-Tensor whole(const Tensor& t) {
-  Tensor c = t.contiguous();
-  return aligned16(c) ? c : c.clone();
-}
-
 struct GroupedFn : torch::autograd::Function<GroupedFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& xIn, const Tensor& wIn, const Tensor& ends) {
     Below below;
@@ -364,6 +351,7 @@ void bindOps(py::module_& m) {
 PYBIND11_MODULE(mccl_torch, m) {
   mccl_torch::bindOps(m);
   mccl_torch::bindComm(m);
+  mccl_torch::bindFp8(m);
   mccl_torch::bindMoe(m);
   mccl_torch::bindGpt2(m);
   mccl_torch::bindLlama(m);
