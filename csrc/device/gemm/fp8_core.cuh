@@ -47,7 +47,7 @@ template <int BN> struct Smem {
   static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
   static constexpr int SCALE_BYTES = 512 + BN * 4;         // a set: 128 words of A, BN of B
   static constexpr int TABLE_BYTES = 2 * (grouped::kMaxGroups + 4) * 4;
-  static constexpr int TOTAL = TILE_BYTES + kScaleSets * SCALE_BYTES + TABLE_BYTES + 256 + 1024;
+  static constexpr int TOTAL = TILE_BYTES + kEpiWarps * grouped::kStageBytes + kScaleSets * SCALE_BYTES + TABLE_BYTES + 256 + 1024;
 };
 
 // Scales in shared memory, 32 rows of 16 bytes, as tcgen05.cp reads them: no swizzle, groups of eight rows 128 bytes apart.
@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
   uint8_t* sB = smem + ST * S::A_BYTES;
-  uint8_t* sScale = smem + S::TILE_BYTES;
+  uint8_t* sStage = smem + S::TILE_BYTES;
+  uint8_t* sScale = sStage + kEpiWarps * grouped::kStageBytes;
   int* table = reinterpret_cast<int*>(sScale + kScaleSets * S::SCALE_BYTES);
   const Groups g{table, table + grouped::kMaxGroups + 4};
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + S::TABLE_BYTES);
@@ -228,9 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
       __syncwarp();
       if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);    // the sums are in registers: the next tile may start
       if (++acc == ACCS) { acc = 0; accPhase ^= 1; }
-      const int r = tile.row + q * 32 + lane;
-      if (r < g.start[tile.e + 1] - g.start[tile.e])
-        grouped::storeColumns<COLS>(v, a.out + ((size_t)g.start[tile.e] + r) * (size_t)a.N, tile.col + half * COLS, a.N);
+      const int r = tile.row + q * 32;
+      grouped::storeTile<COLS>(v, sStage + (warp - 4) * grouped::kStageBytes, a.out + ((size_t)g.start[tile.e] + r) * (size_t)a.N,
+                               g.start[tile.e + 1] - g.start[tile.e] - r, tile.col + half * COLS, a.N, lane);
     }
     grouped::clearRows(a.out, g.start[a.groups], a.rows, a.N);
   }

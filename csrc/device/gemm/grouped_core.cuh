@@ -30,6 +30,7 @@ namespace grouped {
 
 using gemm::BM;
 constexpr int kThreads = 384, kEpiWarps = 8, kMaxGroups = 1024;
+constexpr int kStageBytes = 2048;      // shared memory of an epilogue warp
 constexpr int kStageK = 128;           // bytes of the contracted dimension a stage holds, one swizzled row: 64 bf16
 enum Mode { FORWARD = 0, DATA = 1, WEIGHT = 2 };
 
@@ -51,7 +52,7 @@ template <int BN> struct Smem {
   static constexpr int STAGES = BN == 256 ? 4 : 6;
   static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
   static constexpr int TABLE_BYTES = 2 * (kMaxGroups + 4) * 4;
-  static constexpr int TOTAL = TILE_BYTES + TABLE_BYTES + 256 + 1024;
+  static constexpr int TOTAL = TILE_BYTES + kEpiWarps * kStageBytes + TABLE_BYTES + 256 + 1024;
 };
 
 // MN-major bf16 tile written by TMA with the 128-byte swizzle: chunks of 64 columns, each 64 contracted rows of 128 bytes.
@@ -129,17 +130,32 @@ __device__ __forceinline__ bool waitWarp(uint64_t* bar, uint32_t parity, uint64_
   return false;
 }
 
-// COLS sums of one row, as bf16, to the columns from col0 on of a row of `width`.
+// The epilogue of a warp: 32 rows (lane: row) x COLS sums as bf16, to `rows` rows from `out` on, `width` elements apart, columns from col0
+// on.  32 columns at a time go through 2 KB of shared memory, so that four lanes store 64 bytes of one row: a store from where the
+// sums are, a row per lane, touches 32 lines, and those take the SM longer than the products of a short contraction (64 experts of
+// 128 rows, dw of 2048 x 1024: 133 us; through shared memory 84 us).  16-byte pieces are swizzled over the rows: no bank is hit twice.
 template <int COLS>
-__device__ __forceinline__ void storeColumns(const uint32_t* v, __nv_bfloat16* row, int col0, int width) {
+__device__ __forceinline__ void storeTile(const uint32_t* v, uint8_t* stage, __nv_bfloat16* out, int rows, int col0, int width, int lane) {
 #pragma unroll
-  for (int j = 0; j < COLS / 8; ++j) {
-    if (col0 + j * 8 >= width) break;
-    uint4 o;
-    __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+  for (int c = 0; c < COLS / 32; ++c) {
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o2[i] = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
-    *reinterpret_cast<uint4*>(row + col0 + j * 8) = o;
+    for (int j = 0; j < 4; ++j) {
+      uint4 o;
+      __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o2[i] = __floats2bfloat162_rn(__uint_as_float(v[32 * c + 8 * j + 2 * i]), __uint_as_float(v[32 * c + 8 * j + 2 * i + 1]));
+      *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = o;
+    }
+    __syncwarp();
+    const int col = col0 + 32 * c + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      const uint4 o = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+      if (r < rows && col < width) *reinterpret_cast<uint4*>(out + (size_t)r * width + col) = o;
+    }
   }
 }
 // The epilogue warps' share of the rows behind the last group, which belong to nobody.
@@ -158,8 +174,10 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
   uint8_t* sB = smem + ST * S::A_BYTES;
-  const Groups g{reinterpret_cast<int*>(smem + S::TILE_BYTES), reinterpret_cast<int*>(smem + S::TILE_BYTES) + kMaxGroups + 4};
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::TILE_BYTES + S::TABLE_BYTES);
+  uint8_t* sStage = smem + S::TILE_BYTES;
+  int* table = reinterpret_cast<int*>(sStage + kEpiWarps * kStageBytes);
+  const Groups g{table, table + kMaxGroups + 4};
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + S::TABLE_BYTES);
   uint64_t* full = bars;                                   // [ST] TMA -> MMA
   uint64_t* empty = bars + ST;                             // [ST] MMA -> TMA
   uint64_t* tmemFull = bars + 2 * ST;                      // [2] MMA -> epilogue
@@ -296,10 +314,10 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
         if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
         acc ^= 1; if (acc == 0) accPhase ^= 1;
       }
-      const int r = tile.row + q * 32 + lane;
+      const int r = tile.row + q * 32;
       const int limit = MODE == WEIGHT ? a.tileRows : g.start[tile.e + 1] - g.start[tile.e];
       const size_t row = MODE == WEIGHT ? (size_t)tile.e * a.tileRows + r : (size_t)g.start[tile.e] + r;
-      if (r < limit) storeColumns<COLS>(v, a.out + row * (size_t)a.width, tile.col + half * COLS, a.width);
+      storeTile<COLS>(v, sStage + (warp - 4) * kStageBytes, a.out + row * (size_t)a.width, limit - r, tile.col + half * COLS, a.width, lane);
     }
     if (MODE != WEIGHT) clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }
