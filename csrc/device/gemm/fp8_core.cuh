@@ -60,17 +60,23 @@ __device__ __forceinline__ uint64_t smemDescScales(const void* p) {
   return d;
 }
 // 32 rows x 128 bits from shared memory to four columns of tensor memory, in all four lane quarters.
-__device__ __forceinline__ void copyScales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(desc) : "memory");
+__device__ __forceinline__ void copyScales(uint32_t tmem, uint32_t descLo, uint32_t descHi) {
+  asm volatile("{\n .reg .b64 d;\n mov.b64 d, {%1, %2};\n tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n}" :: "r"(tmem), "r"(descLo), "r"(descHi) : "memory");
 }
-// Instruction descriptor of kind::mxf8f6f4 with e4m3 A and B, both K-major, e8m0 scales, M x N; byte `id` of the scales' words.
+// Instruction descriptor of kind::mxf8f6f4 with e4m3 A and B, both K-major, e8m0 scales, M x N; plus kScaleByte for each byte of the
+// scales' words after the first.
 __host__ __device__ constexpr uint32_t instrDesc(int m, int n) { return ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24); }
-__device__ __forceinline__ void mmaScaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+constexpr uint32_t kScaleByte = (1u << 4) | (1u << 29);
+__device__ __forceinline__ void mmaScaled(uint32_t d, uint32_t aLo, uint32_t bLo, uint32_t hi, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
-      :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n setp.ne.b32 p, %7, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %4, [%5], [%6], p;\n}"
+      :: "r"(d), "r"(aLo), "r"(bLo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
 }
+
+// With programmatic stream serialization this kernel starts before the one that quantises its rows has ended: nothing of that kernel's is
+// read before this.  Without, it returns at once.
+__device__ __forceinline__ void waitForPredecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Scales of blocks [4 i, 4 i + 4) of a row, of which there are `blocks`.
 __device__ __forceinline__ uint32_t scaleWord(const uint8_t* row, int i, int blocks) {
@@ -130,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer
     int stage = 0, e = 0; uint32_t phase = 0;
+    waitForPredecessor();
     for (int t = blockIdx.x; t < totalTiles && *sFail == 0; t += gridDim.x) {
       Tile tile;
       at(t, &e, &tile);
@@ -142,47 +149,57 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
     }
-  } else if (warp == 1 && lane == 0) {
-    // ---------------- MMA issuer
+  } else if (warp == 1) {
+    // ---------------- MMA issuer: the warp walks the loop together, one thread of it issues
+    const bool issues = umma::electOne();
+    const uint64_t descA = umma::smemDescSw128(sA), descScale = smemDescScales(sScale);
+    const uint32_t aLo0 = (uint32_t)descA, bLo0 = (uint32_t)umma::smemDescSw128(sB), hi = (uint32_t)(descA >> 32);
+    const uint32_t scaleLo0 = (uint32_t)descScale, scaleHi = (uint32_t)(descScale >> 32);
     int stage = 0, e = 0, acc = 0, set = 0; uint32_t phase = 0, accPhase = 0, setPhase = 0;
-    for (int t = blockIdx.x; t < totalTiles && *sFail == 0; t += gridDim.x) {
+    for (int t = blockIdx.x; t < totalTiles; t += gridDim.x) {
       Tile tile;
       at(t, &e, &tile);
-      if (!umma::mbarWait(&tmemEmpty[acc], accPhase ^ 1, budget)) { *sFail = 1; atomicExch(a.errFlag, 42); break; }
+      if (!grouped::waitWarp<false>(&tmemEmpty[acc], accPhase ^ 1, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 42); break; }
       umma::tcFenceAfter();
       const uint32_t d = tmemBase + (uint32_t)acc * 128u;
       bool ok = true;
-      for (int kb = 0; kb < kBlocks; ++kb) {
+      for (int kb = 0; kb < kBlocks && ok; ++kb) {
         const uint32_t sfa = tmemBase + kScaleBase + (uint32_t)(set * kScaleCols), sfb = sfa + 4;
         if ((kb & 3) == 0) {
-          if (!umma::mbarWait(&scaleFull[set], setPhase, budget)) { ok = false; *sFail = 1; atomicExch(a.errFlag, 43); break; }
+          ok = umma::mbarWait(&scaleFull[set], setPhase, budget);
           umma::tcFenceAfter();
-          const uint8_t* from = sScale + set * S::SCALE_BYTES;
-          copyScales(sfa, smemDescScales(from));
+          if (issues) {
+            const uint32_t from = scaleLo0 + (uint32_t)(set * (S::SCALE_BYTES >> 4));
+            copyScales(sfa, from, scaleHi);
 #pragma unroll
-          for (int b = 0; b < BN / 128; ++b) copyScales(sfb + 4 * b, smemDescScales(from + 512 + 512 * b));
+            for (int b = 0; b < BN / 128; ++b) copyScales(sfb + 4 * b, from + 32 + 32 * b, scaleHi);
+          }
         }
-        if (!umma::mbarWait(&full[stage], phase, budget)) { ok = false; *sFail = 1; atomicExch(a.errFlag, 44); break; }
+        ok = umma::mbarWait(&full[stage], phase, budget) && ok;
         umma::tcFenceAfter();
-        const uint64_t da = umma::smemDescSw128(sA + stage * S::A_BYTES), db = umma::smemDescSw128(sB + stage * S::B_BYTES);
-        const uint32_t id = (uint32_t)(kb & 3), idesc = instrDesc(BM, BN) | (id << 4) | (id << 29);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mmaScaled(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, sfa, sfb, (kb | k) != 0);
-        umma::mmaCommit(&empty[stage]);
-        if ((kb & 3) == 3 || kb == kBlocks - 1) {
-          umma::mmaCommit(&scaleEmpty[set]);
-          if (++set == kScaleSets) { set = 0; setPhase ^= 1; }
+        const bool lastOfSet = (kb & 3) == 3 || kb == kBlocks - 1;
+        if (issues) {
+          const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));
+          const uint32_t idesc = instrDesc(BM, BN) + (uint32_t)(kb & 3) * kScaleByte;
+          mmaScaled(d, aLo, bLo, hi, idesc, sfa, sfb, kb != 0);
+          mmaScaled(d, aLo + 2, bLo + 2, hi, idesc, sfa, sfb, 1);
+          mmaScaled(d, aLo + 4, bLo + 4, hi, idesc, sfa, sfb, 1);
+          mmaScaled(d, aLo + 6, bLo + 6, hi, idesc, sfa, sfb, 1);
+          umma::mmaCommit(&empty[stage]);
+          if (lastOfSet) umma::mmaCommit(&scaleEmpty[set]);
         }
+        if (lastOfSet && ++set == kScaleSets) { set = 0; setPhase ^= 1; }
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
-      if (!ok) break;
-      umma::mmaCommit(&tmemFull[acc]);
+      if (!__all_sync(0xffffffffu, ok)) { *sFail = 1; if (lane == 0) atomicExch(a.errFlag, 44); break; }
+      if (issues) umma::mmaCommit(&tmemFull[acc]);
       if (++acc == ACCS) { acc = 0; accPhase ^= 1; }
     }
   } else if (warp == 3) {
     // ---------------- scales
     int set = 0, e = 0; uint32_t setPhase = 0;
     bool ok = true;
+    waitForPredecessor();
     for (int t = blockIdx.x; t < totalTiles && ok; t += gridDim.x) {
       Tile tile;
       at(t, &e, &tile);
@@ -236,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
     grouped::clearRows(a.out, g.start[a.groups], a.rows, a.N);
   }
 
+  waitForPredecessor();                                    // this grid's end stands for its predecessor's too
   umma::tcFenceBefore();
   __syncthreads();
   if (warp == 2) umma::tmemDealloc(tmemBase, gemm::kTmemCols);

@@ -15,43 +15,33 @@ using namespace mccl::fp8;
 
 namespace {
 
-// Bytes [outer][rows][cols] (outer 0: a matrix), rows `ld` apart; box = 128 columns x boxRows.  Elements outside read as zero.
-mcclResult_t mapOf(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxRows) {
-  static gemm::EncodeTiledFn fn = gemm::encodeTiled();
-  if (fn == nullptr) MCCLFAIL(mcclSystemError);
-  const cuuint64_t dims[3] = {cols, rows, outer};
-  const cuuint64_t strides[2] = {ld, rows * ld};
-  const cuuint32_t box[3] = {kBlock, boxRows, 1}, elemStrides[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, outer ? 3 : 2, const_cast<void*>(base), dims, strides, box, elemStrides,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    MCCL_WARN("cuTensorMapEncodeTiled failed with %d (base %p, %llu x %llu x %llu bytes, row pitch %llu)", (int)r, base, (unsigned long long)outer,
-              (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)ld);
-    return mcclInvalidArgument;
-  }
-  return mcclSuccess;
-}
-
 template <int BN>
-mcclResult_t launchAs(const Args& a, int dev, int grid, cudaStream_t s) {
+mcclResult_t launchAs(const Args& a, int dev, int grid, bool behind, cudaStream_t s) {
   auto* kernel = fp8Kernel<BN>;
   static std::atomic<uint64_t> prepared{0};                // a bit per device: the attribute stays with the function
   if (!(prepared.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BN>::TOTAL) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
     prepared.fetch_or(1ull << (dev & 63));
   }
-  kernel<<<grid, kThreads, Smem<BN>::TOTAL, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? mcclSuccess : mcclSystemError;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem<BN>::TOTAL;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = behind ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
+  return mcclSuccess;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-}  // namespace
-
-extern "C" {
-
-mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t ldxScale, const void* w, const void* wScale, int64_t ldwScale, void* y,
-                         const void* ends, int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream) {
+// x: e4m3 with its scales; `behind`: made by the kernel launched last on the stream, which lets this one start before that has ended.
+mcclResult_t product(const void* x, int64_t ldx, const void* xScale, int64_t ldxScale, const void* w, const void* wScale, int64_t ldwScale, void* y,
+                     const void* ends, int ends64, int groups, int64_t rows, int N, int K, bool behind, mcclStream_t stream) {
   const int kb = (K + kBlock - 1) / kBlock;
   if (groups <= 0 || groups > grouped::kMaxGroups || (ends == nullptr && groups != 1) || rows < 0 || rows > INT32_MAX - 256 || N <= 0 || K <= 0 ||
       N > INT32_MAX - 256 || K > INT32_MAX - 256 || N % 8 || K % 16) return mcclInvalidArgument;
@@ -61,14 +51,16 @@ mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t
   int dev = 0;
   cudaGetDevice(&dev);
   cudaSetDevice(dev);                                      // binds the context to this thread, for the driver's encoder
+  if (gemm::thinWanted(rows, ends != nullptr, groups, N))
+    return gemm::thinGemm(gemm::ThinCall{x, w, ldx, true, xScale, wScale, ldxScale, ldwScale, y, ends, ends64, groups, rows, N, K, behind}, dev, stream);
   const int64_t rowTiles = ends == nullptr ? (rows + BM - 1) / BM : rows / BM + (rows < groups ? rows : groups);
   const int sms = gemm::gemmSmCount(), bn = N > 128 && rowTiles * ((N + 255) / 256) >= sms ? 256 : 128;
   const int64_t tiles = rowTiles * ((N + bn - 1) / bn);
   if (tiles > INT32_MAX) return mcclInvalidArgument;
   Args a;
   memset(&a, 0, sizeof(a));
-  MCCLCHECK(mapOf(&a.mapA, x, 0, rows, K, ldx, BM));
-  MCCLCHECK(mapOf(&a.mapB, w, groups, N, K, K, bn));
+  MCCLCHECK(gemm::rowsMap(&a.mapA, x, 1, 0, rows, K, ldx, BM));
+  MCCLCHECK(gemm::rowsMap(&a.mapB, w, 1, groups, N, K, K, bn));
   a.sx = static_cast<const uint8_t*>(xScale);
   a.sw = static_cast<const uint8_t*>(wScale);
   a.ldsx = ldxScale; a.ldsw = ldwScale;
@@ -79,7 +71,23 @@ mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t
   if (a.errFlag == nullptr) return mcclSystemError;
   a.budgetNs = 2000000000ull;
   const int grid = (int)(tiles < sms ? tiles : sms);
-  return bn == 256 ? launchAs<256>(a, dev, grid, reinterpret_cast<cudaStream_t>(stream)) : launchAs<128>(a, dev, grid, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return bn == 256 ? launchAs<256>(a, dev, grid, behind, s) : launchAs<128>(a, dev, grid, behind, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t ldxScale, const void* w, const void* wScale, int64_t ldwScale, void* y,
+                         const void* ends, int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream) {
+  return product(x, ldx, xScale, ldxScale, w, wScale, ldwScale, y, ends, ends64, groups, rows, N, K, false, stream);
+}
+
+mcclResult_t mcclFp8GemmBf16Rows(const void* x, int64_t ldx, void* q, void* qScale, int64_t ldqScale, const void* w, const void* wScale, int64_t ldwScale,
+                                 void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream) {
+  MCCLCHECK(mcclFp8QuantizeRows(x, ldx, q, qScale, ldqScale, rows, K, stream));
+  return product(q, K, qScale, ldqScale, w, wScale, ldwScale, y, ends, ends64, groups, rows, N, K, rows > 0, stream);
 }
 
 }  // extern "C"

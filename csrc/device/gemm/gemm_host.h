@@ -19,5 +19,27 @@ int* gemmErrFlag(int device);
 // Multiprocessors of the current device.
 int gemmSmCount();
 
+// y [rows, N] = x w^T for few rows (thin_core.cuh): bf16, or e4m3 with scales; ends null: one group.  `behind`: launched right behind the
+// kernel that makes x and its scales, which lets it start early.
+struct ThinCall {
+  const void *x, *w;
+  int64_t ldx;                          // elements
+  bool fp8;
+  const void *sx, *sw;
+  int64_t ldsx, ldsw;
+  void* out;
+  const void* ends;
+  int ends64, groups;
+  int64_t rows;
+  int N, K;
+  bool behind;
+};
+// Whether this many rows are better served by the thin form: where the tiles of 128 rows x 128 columns are no more than the SMs.
+bool thinWanted(int64_t rows, bool ragged, int groups, int N);
+mcclResult_t thinGemm(const ThinCall& c, int device, void* stream);
+// Tensor map of [outer][rows][cols] (outer 0: a matrix) of 2-byte (bf16) or 1-byte elements, rows `ld` elements apart: boxes of 128 bytes x
+// boxRows, 128-byte swizzle, zeros outside.
+mcclResult_t rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxRows);
+
 }  // namespace gemm
 }  // namespace mccl

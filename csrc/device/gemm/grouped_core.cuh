@@ -248,10 +248,13 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer (lane 0; the whole warp clears rows)
+    // ---------------- MMA issuer: the warp walks the loop together and clears rows, one thread of it issues
+    const bool issues = umma::electOne();
     constexpr bool aMn = MODE == WEIGHT, bMn = MODE != FORWARD;
     constexpr uint32_t idesc = umma::instrDescBf16(BM, BN) | (aMn ? 1u << 15 : 0) | (bMn ? 1u << 16 : 0);
     constexpr int aStep = aMn ? 128 : 2, bStep = bMn ? 128 : 2;    // 16 contracted elements on, in 16-byte units
+    const uint64_t descA = aMn ? smemDescMn(sA) : umma::smemDescSw128(sA), descB = bMn ? smemDescMn(sB) : umma::smemDescSw128(sB);
+    const uint32_t aLo0 = (uint32_t)descA, aHi = (uint32_t)(descA >> 32), bLo0 = (uint32_t)descB, bHi = (uint32_t)(descB >> 32);
     int stage = 0, e = 0, acc = 0; uint32_t phase = 0, accPhase = 0;
     for (int t = blockIdx.x; t < totalTiles; t += gridDim.x) {
       Tile tile;
@@ -263,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       const uint32_t d = tmemBase + (uint32_t)acc * 256u;
       bool ok = true;
       for (int kb = 0; kb < blocks; ++kb) {
-        if (!waitWarp<false>(&full[stage], phase, budget, sFail)) { ok = false; if (lane == 0) atomicExch(a.errFlag, 33); break; }
+        ok = umma::mbarWait(&full[stage], phase, budget);
+        if (!ok) break;
         uint8_t *pa = sA + stage * S::A_BYTES, *pb = sB + stage * S::B_BYTES;
         if (MODE == WEIGHT && tail != 0 && kb == blocks - 1) {
           // Rows [tail, 64) of every chunk: whole 128-byte lines, which the swizzle does not mix.
@@ -278,16 +282,18 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
         }
         __syncwarp();
         umma::tcFenceAfter();
-        if (lane == 0) {
-          const uint64_t da = aMn ? smemDescMn(pa) : umma::smemDescSw128(pa), db = bMn ? smemDescMn(pb) : umma::smemDescSw128(pb);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma::mmaBf16(d, da + (uint64_t)(k * aStep), db + (uint64_t)(k * bStep), idesc, (kb | k) != 0);
+        if (issues) {
+          const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));
+          umma::mmaBf16Split(d, aLo, aHi, bLo, bHi, idesc, kb != 0);
+          umma::mmaBf16Split(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
+          umma::mmaBf16Split(d, aLo + 2 * aStep, aHi, bLo + 2 * bStep, bHi, idesc, 1);
+          umma::mmaBf16Split(d, aLo + 3 * aStep, aHi, bLo + 3 * bStep, bHi, idesc, 1);
           umma::mmaCommit(&empty[stage]);
         }
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
-      if (!ok) break;
-      if (lane == 0) umma::mmaCommit(&tmemFull[acc]);
+      if (!__all_sync(0xffffffffu, ok)) { *sFail = 1; if (lane == 0) atomicExch(a.errFlag, 33); break; }
+      if (issues) umma::mmaCommit(&tmemFull[acc]);
       acc ^= 1; if (acc == 0) accPhase ^= 1;
     }
   } else if (warp >= 4) {

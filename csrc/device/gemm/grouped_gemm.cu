@@ -13,18 +13,16 @@
 using namespace mccl;
 using namespace mccl::grouped;
 
-namespace {
-
-// bf16 [outer][rows][cols], rows `ld` elements apart, the outer index rows * ld apart (rank 2: outer = 0); box = boxCols x boxRows,
-// 128 bytes inside.  Elements outside read as zero.
-mcclResult_t mapOf(CUtensorMap* map, const void* base, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxCols, uint32_t boxRows) {
-  static gemm::EncodeTiledFn fn = gemm::encodeTiled();
+mcclResult_t mccl::gemm::rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld,
+                                 uint32_t boxRows) {
+  static EncodeTiledFn fn = encodeTiled();
   if (fn == nullptr) MCCLFAIL(mcclSystemError);
   const cuuint64_t dims[3] = {cols, rows, outer};
-  const cuuint64_t strides[2] = {ld * 2, rows * ld * 2};
-  const cuuint32_t box[3] = {boxCols, boxRows, 1}, elemStrides[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, outer ? 3 : 2, const_cast<void*>(base), dims, strides, box, elemStrides,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t strides[2] = {ld * elementBytes, rows * ld * elementBytes};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / elementBytes), boxRows, 1}, elemStrides[3] = {1, 1, 1};
+  const CUresult r = fn(map, elementBytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, outer ? 3 : 2, const_cast<void*>(base), dims,
+                        strides, box, elemStrides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     MCCL_WARN("cuTensorMapEncodeTiled failed with %d (base %p, %llu x %llu x %llu, row pitch %llu)", (int)r, base, (unsigned long long)outer,
               (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)ld);
@@ -32,6 +30,8 @@ mcclResult_t mapOf(CUtensorMap* map, const void* base, uint64_t outer, uint64_t 
   }
   return mcclSuccess;
 }
+
+namespace {
 
 // The current device, its context bound to this thread: the driver's encoder needs it, and a thread of the autograd engine that has
 // launched nothing yet has none.
@@ -94,13 +94,18 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
   if (!valid(s)) return mcclInvalidArgument;
   if (rows == 0) return mcclSuccess;
   if (!validRows(x, ldx, K) || w == nullptr || y == nullptr || !aligned16(w) || !aligned16(y)) return mcclInvalidArgument;
+  const int dev = boundDevice();
+  if (gemm::thinWanted(rows, true, groups, N)) {
+    gemm::ThinCall c{};
+    c.x = x; c.w = w; c.ldx = ldx; c.out = y; c.ends = ends; c.ends64 = ends64; c.groups = groups; c.rows = rows; c.N = N; c.K = K;
+    return gemm::thinGemm(c, dev, stream);
+  }
   Args a;
   memset(&a, 0, sizeof(a));
-  const int dev = boundDevice();
   const int64_t rt = rowTilesAtMost(s);
   const int bn = pickColumns(rt, N, gemm::gemmSmCount());
-  MCCLCHECK(mapOf(&a.mapA, x, 0, rows, K, ldx, 64, BM));
-  MCCLCHECK(mapOf(&a.mapB, w, groups, N, K, K, 64, bn));
+  MCCLCHECK(gemm::rowsMap(&a.mapA, x, 2, 0, rows, K, ldx, BM));
+  MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, bn));
   a.contracted = K; a.width = N;
   a.out = static_cast<__nv_bfloat16*>(y);
   return run<FORWARD>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
@@ -117,8 +122,8 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
   const int dev = boundDevice();
   const int64_t rt = rowTilesAtMost(s);
   const int bn = pickColumns(rt, K, gemm::gemmSmCount());
-  MCCLCHECK(mapOf(&a.mapA, dy, 0, rows, N, lddy, 64, BM));
-  MCCLCHECK(mapOf(&a.mapB, w, groups, N, K, K, 64, 64));
+  MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, BM));
+  MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, 64));
   a.contracted = N; a.width = K;
   a.out = static_cast<__nv_bfloat16*>(dx);
   return run<DATA>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
@@ -136,8 +141,8 @@ mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const v
   const int dev = boundDevice();
   const int64_t rt = (int64_t)groups * ((N + BM - 1) / BM);
   const int bn = pickColumns(rt, K, gemm::gemmSmCount());
-  MCCLCHECK(mapOf(&a.mapA, dy, 0, rows, N, lddy, 64, 64));
-  MCCLCHECK(mapOf(&a.mapB, x, 0, rows, K, ldx, 64, 64));
+  MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, 64));
+  MCCLCHECK(gemm::rowsMap(&a.mapB, x, 2, 0, rows, K, ldx, 64));
   a.tileRows = N; a.width = K;
   a.out = static_cast<__nv_bfloat16*>(dw);
   return run<WEIGHT>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);

@@ -1,0 +1,87 @@
+// Host side of the products with few rows (thin_core.cuh): choice of the tile and of the CTAs that share one, launch.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <string.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../../core/core.h"
+#include "gemm_host.h"
+#include "thin_core.cuh"
+
+using namespace mccl;
+using namespace mccl::thin;
+
+namespace {
+
+template <int BT, bool FP8>
+mcclResult_t launchAs(Args& a, const gemm::ThinCall& c, int dev, int tiles, int shares, int slices, cudaStream_t s) {
+  auto* kernel = thinKernel<BT, FP8>;
+  static std::atomic<uint64_t> prepared{0};                // a bit per device: the attribute stays with the function
+  if (!(prepared.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BT>::TOTAL) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
+    prepared.fetch_or(1ull << (dev & 63));
+  }
+  MCCLCHECK(gemm::rowsMap(&a.mapX, c.x, FP8 ? 1 : 2, 0, c.rows, c.K, c.ldx, BT));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * slices), (unsigned)c.groups, (unsigned)shares);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem<BT>::TOTAL;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = slices; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = c.behind ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
+  return mcclSuccess;
+}
+
+template <bool FP8>
+mcclResult_t launch(int bt, Args& a, const gemm::ThinCall& c, int dev, int tiles, int shares, int slices, cudaStream_t s) {
+  switch (bt) {
+    case 16: return launchAs<16, FP8>(a, c, dev, tiles, shares, slices, s);
+    case 32: return launchAs<32, FP8>(a, c, dev, tiles, shares, slices, s);
+    case 64: return launchAs<64, FP8>(a, c, dev, tiles, shares, slices, s);
+    default: return launchAs<128, FP8>(a, c, dev, tiles, shares, slices, s);
+  }
+}
+
+int64_t expertsWithRows(int64_t rows, int groups) { return std::min<int64_t>(rows, groups); }
+
+}  // namespace
+
+bool mccl::gemm::thinWanted(int64_t rows, bool ragged, int groups, int N) {
+  const int64_t rowTiles = ragged ? rows / BM + expertsWithRows(rows, groups) : (rows + BM - 1) / BM;
+  return rowTiles * ((N + BM - 1) / BM) <= gemmSmCount();
+}
+
+mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
+  const bool ragged = c.ends != nullptr;
+  const int sms = gemmSmCount(), nTiles = (c.N + BM - 1) / BM;
+  // Rows of a tile: those of a group where they are known, twice the mean where not.
+  const int64_t experts = ragged ? expertsWithRows(c.rows, c.groups) : 1, rows = ragged ? 2 * ((c.rows + experts - 1) / experts) : c.rows;
+  const int bt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const int64_t shares = ragged ? 1 : (c.rows + bt - 1) / bt;
+  // CTAs a tile: as many as the SMs hold at a time, two an SM up to 64 rows.
+  const int perUnit = c.fp8 ? 512 : 64, units = (c.K + perUnit - 1) / perUnit;
+  const int64_t places = (int64_t)sms * (bt <= 64 ? 2 : 1), tiles = (int64_t)nTiles * c.groups * shares;       // those of experts without rows start, too
+  const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8, places / tiles, units}));
+  Args a;
+  memset(&a, 0, sizeof(a));
+  MCCLCHECK(rowsMap(&a.mapW, c.w, c.fp8 ? 1 : 2, c.groups, c.N, c.K, c.K, BM));
+  a.sx = static_cast<const uint8_t*>(c.sx);
+  a.sw = static_cast<const uint8_t*>(c.sw);
+  a.ldsx = c.ldsx; a.ldsw = c.ldsw;
+  a.ends = c.ends; a.ends64 = c.ends64; a.groups = c.groups;
+  a.rows = (int)c.rows; a.N = c.N; a.K = c.K; a.slices = slices;
+  a.out = static_cast<__nv_bfloat16*>(c.out);
+  a.errFlag = gemmErrFlag(device);
+  if (a.errFlag == nullptr) return mcclSystemError;
+  a.budgetNs = 2000000000ull;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return c.fp8 ? launch<true>(bt, a, c, device, nTiles, (int)shares, slices, s) : launch<false>(bt, a, c, device, nTiles, (int)shares, slices, s);
+}

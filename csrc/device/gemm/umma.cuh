@@ -126,6 +126,21 @@ __device__ __forceinline__ void mmaBf16(uint32_t tmemD, uint64_t descA, uint64_t
       " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
       :: "r"(tmemD), "l"(descA), "l"(descB), "r"(idesc), "r"(accumulate) : "memory");
 }
+// One thread of a converged warp.  A warp that walks its loop together and issues under this predicate keeps descriptors and addresses in
+// uniform registers; a branch taken by one lane has each of them moved there again for every instruction (64 stages of four small MMAs
+// in a row: 0.42 us a stage by a lane's branch, 0.27 by an elected thread).
+__device__ __forceinline__ bool electOne() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+// mmaBf16 with the descriptors given as low words and one high word: steps along K only change the low word.
+__device__ __forceinline__ void mmaBf16Split(uint32_t tmemD, uint32_t aLo, uint32_t aHi, uint32_t bLo, uint32_t bHi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n}"
+      :: "r"(tmemD), "r"(aLo), "r"(aHi), "r"(bLo), "r"(bHi), "r"(idesc), "r"(accumulate) : "memory");
+}
 // Arrive on `bar` once every MMA issued so far by this thread has completed.
 __device__ __forceinline__ void mmaCommit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smemAddr(bar)) : "memory");

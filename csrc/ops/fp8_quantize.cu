@@ -48,6 +48,7 @@ __device__ __forceinline__ uint2 quantize(const uint4& q, uint32_t byte) {
 // Sixteen threads a block of 128; the threads of a grid walk the blocks of all rows.
 __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, uint8_t* scale, int64_t lds, int64_t rows, int K,
                                                                int blocks) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // a product behind this may start; it waits for this grid's end where it reads
   const int64_t b = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4, total = rows * blocks;
   const int in = (threadIdx.x & 15) * 8;
   const int64_t row = b < total ? b / blocks : 0;

@@ -25,13 +25,9 @@ Tensor scaleRows(const Tensor& s) {
 
 struct Quantized { Tensor data, scale; };       // scale: bytes
 
-Quantized quantizeRows(const Tensor& xIn) {
-  Tensor x = alignedRows(xIn);
+Quantized quantizedLike(const Tensor& x) {
   const int64_t M = x.size(0), K = x.size(1);
-  Quantized r{at::empty({M, K}, x.options().dtype(at::kFloat8_e4m3fn)), scaleStore({M, blocksOf(K)}, x)};
-  check(mcclFp8QuantizeRows(x.data_ptr(), pitchOf(x), r.data.data_ptr(), r.scale.data_ptr(), r.scale.stride(0), M, (int)K, streamOf(x)), "mcclFp8QuantizeRows");
-  counters().gemm += M > 0;
-  return r;
+  return {at::empty({M, K}, x.options().dtype(at::kFloat8_e4m3fn)), scaleStore({M, blocksOf(K)}, x)};
 }
 
 // e4m3 values and e8m0 scales of bf16 x: [M, K] by blocks of 128 of a row, or (tiles) [.., N, K] by 128 x 128.
@@ -40,7 +36,11 @@ std::pair<Tensor, Tensor> fp8Quantize(const Tensor& xIn, bool tiles) {
   Below below;
   c10::cuda::CUDAGuard guard(xIn.device());
   if (!tiles) {
-    Quantized r = quantizeRows(xIn);
+    Tensor x = alignedRows(xIn);
+    Quantized r = quantizedLike(x);
+    check(mcclFp8QuantizeRows(x.data_ptr(), pitchOf(x), r.data.data_ptr(), r.scale.data_ptr(), r.scale.stride(0), x.size(0), (int)x.size(1), streamOf(x)),
+          "mcclFp8QuantizeRows");
+    counters().gemm += x.size(0) > 0;
     return {r.data, r.scale.view(at::kFloat8_e8m0fnu)};
   }
   Tensor x = whole(xIn);
@@ -59,12 +59,21 @@ Tensor fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const Tenso
   TORCH_CHECK(!recorded() && ordinary(x) && ordinary(wIn), "fp8_gemm: not under tracing, a dispatch mode or torch.func");
   Below below;
   c10::cuda::CUDAGuard guard(x.device());
-  Quantized a = xScale ? Quantized{alignedRows(x), scaleRows(*xScale)} : quantizeRows(x);
-  Tensor w = whole(wIn), ws = scaleRows(wScale);
+  Tensor rows = alignedRows(x), w = whole(wIn), ws = scaleRows(wScale);
   const int64_t M = x.size(0), K = x.size(1), N = w.size(-2), E = w.dim() == 3 ? w.size(0) : 1;
   Tensor y = at::empty({M, N}, x.options().dtype(at::kBFloat16));
-  check(mcclFp8Gemm(a.data.data_ptr(), pitchOf(a.data), a.scale.data_ptr(), a.scale.stride(0), w.data_ptr(), ws.data_ptr(), ws.stride(-2), y.data_ptr(),
-                    ends ? ends->data_ptr() : nullptr, ends && ends->scalar_type() == at::kLong, (int)E, M, (int)N, (int)K, streamOf(x)), "mcclFp8Gemm");
+  const void* e = ends ? ends->data_ptr() : nullptr;
+  const int wide = ends && ends->scalar_type() == at::kLong;
+  if (xScale) {
+    Tensor xs = scaleRows(*xScale);
+    check(mcclFp8Gemm(rows.data_ptr(), pitchOf(rows), xs.data_ptr(), xs.stride(0), w.data_ptr(), ws.data_ptr(), ws.stride(-2), y.data_ptr(), e, wide, (int)E, M,
+                      (int)N, (int)K, streamOf(x)), "mcclFp8Gemm");
+  } else {
+    Quantized q = quantizedLike(rows);
+    check(mcclFp8GemmBf16Rows(rows.data_ptr(), pitchOf(rows), q.data.data_ptr(), q.scale.data_ptr(), q.scale.stride(0), w.data_ptr(), ws.data_ptr(),
+                              ws.stride(-2), y.data_ptr(), e, wide, (int)E, M, (int)N, (int)K, streamOf(x)), "mcclFp8GemmBf16Rows");
+    counters().gemm += M > 0;
+  }
   counters().gemm += M > 0;
   return y;
 }

@@ -45,6 +45,10 @@ mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const v
  * group) as in mcclGroupedGemm.  N a multiple of 8, K and ldx of 16; values 16-byte, scales 4-byte aligned. */
 mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t ldxScale, const void* w, const void* wScale, int64_t ldwScale,
                          void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream);
+/* The same for bf16 x [rows, K] (16-byte aligned, ldx a multiple of 8), quantised into q [rows, K] and its scales first. */
+mcclResult_t mcclFp8GemmBf16Rows(const void* x, int64_t ldx, void* q, void* qScale, int64_t ldqScale, const void* w, const void* wScale,
+                                 int64_t ldwScale, void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K,
+                                 mcclStream_t stream);
 /* The smallest scale that brings a block's largest magnitude to 448 or less (a block of zeros: 1), and the nearest e4m3 numbers, of bf16
  * x [rows, K] by blocks of 128 of a row, and of contiguous x [outer, rows, K] by 128 x 128; q contiguous.  What is not finite becomes NaN. */
 mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, void* scale, int64_t ldScale, int64_t rows, int K, mcclStream_t stream);

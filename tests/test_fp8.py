@@ -135,7 +135,7 @@ def _product(x, w, y):
 
 
 SHAPES = [(1, 8, 16), (1, 128, 128), (2, 136, 144), (16, 256, 512), (17, 264, 528), (33, 512, 640), (64, 1032, 2064), (65, 128, 4096), (100, 11008, 256),
-          (128, 520, 1024), (129, 776, 1040), (300, 1024, 2048), (1000, 200, 656), (2049, 2056, 528), (5, 8, 8192), (1, 5504, 4096), (640, 2048, 128)]
+          (128, 520, 1024), (129, 776, 1040), (300, 1024, 2048), (1000, 200, 656), (2049, 2056, 528), (5, 8, 8192), (1, 5504, 4096), (640, 2048, 128), (1500, 2000, 1040), (4100, 1024, 272), (3, 2048, 400), (400, 136, 8192), (1, 11008, 4096)]
 
 
 @pytest.mark.gpu
@@ -156,7 +156,8 @@ def test_rows_in_bf16_are_quantised_within_the_call():
 
 
 GROUPS = [([1], 64, 128), ([2, 0, 1], 136, 144), ([0, 5, 0, 130, 1, 0], 64, 272), ([127, 128, 129, 256, 257], 264, 400), ([33] * 70, 192, 128),
-          ([1024, 3, 2048], 512, 512), ([1] * 9, 2056, 256), ([16, 0, 48, 33], 520, 2064), ([700, 20], 1024, 1296)]
+          ([1024, 3, 2048], 512, 512), ([1] * 9, 2056, 256), ([16, 0, 48, 33], 520, 2064), ([700, 20], 1024, 1296), ([127, 128, 129, 256, 257], 4104, 144),
+          ([1024, 3, 2048, 0, 700], 1032, 528), ([1, 0, 2, 140], 8200, 1008), ([300, 0, 1], 136, 8192)]
 
 
 @pytest.mark.gpu

@@ -58,7 +58,8 @@ def _seed():
 
 CASES = [([1], 8, 8), ([1], 64, 64), ([2, 0, 1], 72, 136), ([0, 5, 0, 130, 1, 0], 64, 64), ([127, 128, 129, 256, 257], 136, 264), ([300], 1032, 264),
          ([63, 64, 65, 1, 0, 191], 520, 776), ([700, 20], 256, 1024), ([33] * 70, 128, 192), ([1024, 3, 2048], 512, 512), ([5, 9], 2048, 64),
-         ([17], 8, 2048), ([1] * 9, 256, 2056), ([16, 0, 48, 33], 2064, 520)]
+         ([17], 8, 2048), ([1] * 9, 256, 2056), ([16, 0, 48, 33], 2064, 520), ([127, 128, 129, 256, 257], 136, 4104), ([1024, 3, 2048, 0, 700], 520, 1032),
+         ([1, 0, 2, 140], 1000, 8200), ([300, 0, 1], 8192, 136), ([128] * 30, 64, 640)]
 
 
 @pytest.mark.gpu
