@@ -34,12 +34,12 @@ struct Args {
 
 template <int BT> struct Smem {
   static constexpr int A_BYTES = BM * 128, B_BYTES = BT * 128;
-  static constexpr int STAGES = BT == 16 ? 5 : BT == 32 ? 4 : BT == 64 ? 3 : 4;      // two CTAs an SM up to 64 rows
+  static constexpr int STAGES = BT == 16 ? 5 : BT == 32 ? 4 : 3;                     // two CTAs an SM
   static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
   static constexpr int SUM_BYTES = BT * BM * 4;
   static constexpr int SCALE_BYTES = 1024;                 // a set: 512 of the weights, 512 of the rows
   static constexpr int TOTAL = TILE_BYTES + SUM_BYTES + fp8::kScaleSets * SCALE_BYTES + 256 + 1024;
-  static constexpr int TMEM = BT <= 32 ? 64 : BT == 64 ? 128 : 256;                  // BT columns of sums and 24 of scales
+  static constexpr int TMEM = BT <= 32 ? 64 : 128;         // BT columns of sums and 24 of scales
 };
 
 __device__ __forceinline__ void arriveCluster(uint64_t* bar, uint32_t cta) {
@@ -74,7 +74,7 @@ __device__ __forceinline__ void tmemLoad32x16(uint32_t taddr, uint32_t* v) {
 using fp8::waitForPredecessor;
 
 template <int BT, bool FP8>
-__global__ void __launch_bounds__(kThreads, BT <= 64 ? 2 : 1) thinKernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant__ Args a) {
   using S = Smem<BT>;
   constexpr int ST = S::STAGES, CK = FP8 ? 128 : 64, UNIT = FP8 ? 4 : 1;             // a rank's share is whole words of scales
   extern __shared__ uint8_t smemRaw[];

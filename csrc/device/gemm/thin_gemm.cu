@@ -45,8 +45,7 @@ mcclResult_t launch(int bt, Args& a, const gemm::ThinCall& c, int dev, int tiles
   switch (bt) {
     case 16: return launchAs<16, FP8>(a, c, dev, tiles, shares, slices, s);
     case 32: return launchAs<32, FP8>(a, c, dev, tiles, shares, slices, s);
-    case 64: return launchAs<64, FP8>(a, c, dev, tiles, shares, slices, s);
-    default: return launchAs<128, FP8>(a, c, dev, tiles, shares, slices, s);
+    default: return launchAs<64, FP8>(a, c, dev, tiles, shares, slices, s);
   }
 }
 
@@ -64,11 +63,11 @@ mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
   const int sms = gemmSmCount(), nTiles = (c.N + BM - 1) / BM;
   // Rows of a tile: those of a group where they are known, twice the mean where not.
   const int64_t experts = ragged ? expertsWithRows(c.rows, c.groups) : 1, rows = ragged ? 2 * ((c.rows + experts - 1) / experts) : c.rows;
-  const int bt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  const int64_t shares = ragged ? 1 : (c.rows + bt - 1) / bt;
-  // CTAs a tile: as many as the SMs hold at a time, two an SM up to 64 rows.
+  const int bt = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  const int64_t shares = (rows + bt - 1) / bt;             // an expert with more rows than expected walks them in turns
+  // CTAs a tile: as many as the SMs hold at a time, two an SM.
   const int perUnit = c.fp8 ? 512 : 64, units = (c.K + perUnit - 1) / perUnit;
-  const int64_t places = (int64_t)sms * (bt <= 64 ? 2 : 1), tiles = (int64_t)nTiles * c.groups * shares;       // those of experts without rows start, too
+  const int64_t places = 2ll * sms, tiles = (int64_t)nTiles * c.groups * shares;       // those of experts without rows start, too
   const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8, places / tiles, units}));
   Args a;
   memset(&a, 0, sizeof(a));

@@ -45,23 +45,43 @@ __device__ __forceinline__ uint2 quantize(const uint4& q, uint32_t byte) {
   return make_uint2(four(q.x, q.y, inv), four(q.z, q.w, inv));
 }
 
-// Sixteen threads a block of 128; the threads of a grid walk the blocks of all rows.
+// Eight threads a block of 128, sixteen values each, four blocks a thread.  8192 x 8192: with sixteen threads a block and one block in
+// flight a thread 55 us, with four 47 us, with eight threads a block 37 us (5.4 TB/s).
+// I: the type the blocks of all rows are counted in (a 64-bit division costs as much as the rest).
+constexpr int kPieces = 4, kPerBlock = 8;
+template <class I>
 __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, uint8_t* scale, int64_t lds, int64_t rows, int K,
                                                                int blocks) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // a product behind this may start; it waits for this grid's end where it reads
-  const int64_t b = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4, total = rows * blocks;
-  const int in = (threadIdx.x & 15) * 8;
-  const int64_t row = b < total ? b / blocks : 0;
-  const int blk = (int)(b - row * blocks), col = blk * kBlock + in;
-  const bool live = b < total && col < K;
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (live) v = *reinterpret_cast<const uint4*>(x + row * ldx + col);
-  uint32_t a = largest(v);
+  const I total = (I)rows * (I)blocks, b0 = (I)blockIdx.x * (kThreads / kPerBlock * kPieces) + (threadIdx.x / kPerBlock);
+  const int in = (threadIdx.x % kPerBlock) * 16;
+  uint4 v[kPieces][2];
+  int64_t row[kPieces];
+  int blk[kPieces];
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const uint32_t byte = scaleByte(a);
-  if (live) *reinterpret_cast<uint2*>(q + row * K + col) = quantize(v, byte);
-  if (b < total && in == 0) scale[row * lds + blk] = (uint8_t)byte;
+  for (int u = 0; u < kPieces; ++u) {
+    const I b = b0 + (I)(u * (kThreads / kPerBlock)), r = b < total ? b / (I)blocks : 0;
+    row[u] = (int64_t)r;
+    blk[u] = b < total ? (int)(b - r * (I)blocks) : -1;
+    const int col = blk[u] * kBlock + in;                  // K is a multiple of 16: all sixteen or none
+    const uint4* from = reinterpret_cast<const uint4*>(x + row[u] * ldx + col);
+    const bool live = blk[u] >= 0 && col < K;
+    v[u][0] = live ? from[0] : make_uint4(0, 0, 0, 0);
+    v[u][1] = live ? from[1] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    uint32_t a = max(largest(v[u][0]), largest(v[u][1]));
+#pragma unroll
+    for (int o = kPerBlock / 2; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const uint32_t byte = scaleByte(a);
+    const int col = blk[u] * kBlock + in;
+    if (blk[u] >= 0 && col < K) {
+      const uint2 lo = quantize(v[u][0], byte), hi = quantize(v[u][1], byte);
+      *reinterpret_cast<uint4*>(q + row[u] * K + col) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+    if (blk[u] >= 0 && in == 0) scale[row[u] * lds + blk[u]] = (uint8_t)byte;
+  }
 }
 
 // One CTA a block of 128 x 128: each thread eight rows' pieces of eight values.
@@ -106,9 +126,10 @@ mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, void* scal
   if (rows < 0 || K <= 0 || K > INT32_MAX - 256 || K % 16 || ldx < K || ldx % 8 || ldScale < blocks) return mcclInvalidArgument;
   if (rows == 0) return mcclSuccess;
   if (!x || !q || !scale || !aligned16(x) || !aligned16(q) || rows * blocks > (int64_t)INT32_MAX * 16) return mcclInvalidArgument;
-  const int64_t ctas = (rows * blocks + kThreads / 16 - 1) / (kThreads / 16);
-  quantizeRowsKernel<<<(unsigned)ctas, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q),
-                                                                                              static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
+  const int64_t per = kThreads / kPerBlock * kPieces, ctas = (rows * blocks + per - 1) / per;
+  auto* kernel = rows * blocks < (1ll << 31) - per ? quantizeRowsKernel<uint32_t> : quantizeRowsKernel<int64_t>;
+  kernel<<<(unsigned)ctas, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q),
+                                                                                  static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
   return launchedOk();
 }
 
