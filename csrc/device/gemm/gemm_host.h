@@ -37,6 +37,20 @@ struct ThinCall {
 // Whether this many rows are better served by the thin form: where the tiles of 128 rows x 128 columns are no more than the SMs.
 bool thinWanted(int64_t rows, bool ragged, int groups, int N);
 mcclResult_t thinGemm(const ThinCall& c, int device, void* stream);
+// The products of groups by pairs of SMs (pair_core.cuh).  mode: 0 y = x w^T, 1 dx = dy w, 2 dw = dy^T x.
+struct PairCall {
+  int mode;
+  const void *a, *b;                    // x or dy; w, or x for mode 2
+  int64_t lda, ldb;                     // elements a row; ldb for mode 2
+  void* out;
+  const void* ends;
+  int ends64, groups;
+  int64_t rows;
+  int N, K;
+};
+// Whether groups of this many rows are better served by pairs.
+bool pairWanted(int mode, int64_t rows, int groups, int N, int K);
+mcclResult_t pairGemm(const PairCall& c, int device, void* stream);
 // Tensor map of [outer][rows][cols] (outer 0: a matrix) of 2-byte (bf16) or 1-byte elements, rows `ld` elements apart: boxes of 128 bytes x
 // boxRows, 128-byte swizzle, zeros outside.
 mcclResult_t rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxRows);

@@ -100,6 +100,8 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
     c.x = x; c.w = w; c.ldx = ldx; c.out = y; c.ends = ends; c.ends64 = ends64; c.groups = groups; c.rows = rows; c.N = N; c.K = K;
     return gemm::thinGemm(c, dev, stream);
   }
+  if (gemm::pairWanted(FORWARD, rows, groups, N, K))
+    return gemm::pairGemm(gemm::PairCall{FORWARD, x, w, ldx, K, y, ends, ends64, groups, rows, N, K}, dev, stream);
   Args a;
   memset(&a, 0, sizeof(a));
   const int64_t rt = rowTilesAtMost(s);
@@ -117,9 +119,11 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
   if (!valid(s)) return mcclInvalidArgument;
   if (rows == 0) return mcclSuccess;
   if (!validRows(dy, lddy, N) || w == nullptr || dx == nullptr || !aligned16(w) || !aligned16(dx)) return mcclInvalidArgument;
+  const int dev = boundDevice();
+  if (gemm::pairWanted(DATA, rows, groups, N, K))
+    return gemm::pairGemm(gemm::PairCall{DATA, dy, w, lddy, K, dx, ends, ends64, groups, rows, N, K}, dev, stream);
   Args a;
   memset(&a, 0, sizeof(a));
-  const int dev = boundDevice();
   const int64_t rt = rowTilesAtMost(s);
   const int bn = pickColumns(rt, K, gemm::gemmSmCount());
   MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, BM));
@@ -136,9 +140,11 @@ mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const v
   if (rows == 0)
     return cudaMemsetAsync(dw, 0, (size_t)groups * N * K * 2, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? mcclSuccess : mcclSystemError;
   if (!validRows(dy, lddy, N) || !validRows(x, ldx, K)) return mcclInvalidArgument;
+  const int dev = boundDevice();
+  if (gemm::pairWanted(WEIGHT, rows, groups, N, K))
+    return gemm::pairGemm(gemm::PairCall{WEIGHT, dy, x, lddy, ldx, dw, ends, ends64, groups, rows, N, K}, dev, stream);
   Args a;
   memset(&a, 0, sizeof(a));
-  const int dev = boundDevice();
   const int64_t rt = (int64_t)groups * ((N + BM - 1) / BM);
   const int bn = pickColumns(rt, K, gemm::gemmSmCount());
   MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, 64));

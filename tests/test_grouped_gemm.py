@@ -59,7 +59,8 @@ def _seed():
 CASES = [([1], 8, 8), ([1], 64, 64), ([2, 0, 1], 72, 136), ([0, 5, 0, 130, 1, 0], 64, 64), ([127, 128, 129, 256, 257], 136, 264), ([300], 1032, 264),
          ([63, 64, 65, 1, 0, 191], 520, 776), ([700, 20], 256, 1024), ([33] * 70, 128, 192), ([1024, 3, 2048], 512, 512), ([5, 9], 2048, 64),
          ([17], 8, 2048), ([1] * 9, 256, 2056), ([16, 0, 48, 33], 2064, 520), ([127, 128, 129, 256, 257], 136, 4104), ([1024, 3, 2048, 0, 700], 520, 1032),
-         ([1, 0, 2, 140], 1000, 8200), ([300, 0, 1], 8192, 136), ([128] * 30, 64, 640)]
+         ([1, 0, 2, 140], 1000, 8200), ([300, 0, 1], 8192, 136), ([128] * 30, 64, 640), ([2051, 1100], 264, 5000), ([2051, 1100], 2600, 1032), ([0, 3000, 77], 1032, 4104),
+         ([2100], 4096, 2056), ([1, 4200, 0, 63], 2048, 2312)]
 
 
 @pytest.mark.gpu
@@ -83,10 +84,10 @@ def test_many_experts():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [5, 200, 1500])
-def test_rows_behind_the_last_group(T):
+@pytest.mark.parametrize("T,K,N", [(5, 200, 328), (200, 200, 328), (1500, 200, 328), (6000, 2600, 2312)])
+def test_rows_behind_the_last_group(T, K, N):
     """They may hold anything, and so may the rows of other groups: no group sees them."""
-    sizes, K, N = [T // 5, 0, T // 3], 200, 328
+    sizes = [T // 5, 0, T // 3]
     used = sum(sizes)
     x, w, dy = _bf(T, K), _bf(3, N, K), _bf(T, N)
     x[used:], dy[used:] = float("nan"), float("inf")
