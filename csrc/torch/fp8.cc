@@ -54,9 +54,23 @@ std::pair<Tensor, Tensor> fp8Quantize(const Tensor& xIn, bool tiles) {
   return {q, s.view(at::kFloat8_e8m0fnu)};
 }
 
-// x: bf16, quantised here, or e4m3 with its scales.  The caller has checked types, shapes and devices.
-Tensor fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const Tensor& wIn, const Tensor& wScale, const std::optional<Tensor>& ends) {
-  TORCH_CHECK(!recorded() && ordinary(x) && ordinary(wIn), "fp8_gemm: not under tracing, a dispatch mode or torch.func");
+// x: bf16, quantised here, or e4m3 with its scales.  None where an argument is not what the kernels take (the caller says which).
+py::object fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const Tensor& wIn, const Tensor& wScale, const std::optional<Tensor>& ends) {
+  constexpr int64_t kMost = INT32_MAX - 256;
+  const int64_t wd = ends ? 3 : 2;
+  if (recorded() || !ordinary(x) || !ordinary(wIn) || !ordinary(wScale) || !x.is_cuda() || x.dim() != 2 || wIn.dim() != wd || wScale.dim() != wd ||
+      wIn.size(wd - 1) != x.size(1)) return py::none();
+  const int64_t n = wIn.size(wd - 2), k = x.size(1);
+  if (n < 1 || n % 8 || k < 1 || k % 16 || x.size(0) >= kMost || n >= kMost || k >= kMost || wIn.scalar_type() != at::kFloat8_e4m3fn ||
+      wScale.scalar_type() != at::kFloat8_e8m0fnu || wScale.size(wd - 2) != blocksOf(n) || wScale.size(wd - 1) != blocksOf(k) || wIn.device() != x.device() ||
+      wScale.device() != x.device()) return py::none();
+  if (ends && (!ordinary(*ends) || (ends->scalar_type() != at::kInt && ends->scalar_type() != at::kLong) || ends->dim() != 1 || !ends->is_contiguous() ||
+               ends->size(0) != wIn.size(0) || wScale.size(0) != wIn.size(0) || wIn.size(0) < 1 || wIn.size(0) > mcclGroupedGemmMaxGroups() ||
+               ends->device() != x.device())) return py::none();
+  if (xScale ? !ordinary(*xScale) || x.scalar_type() != at::kFloat8_e4m3fn || xScale->scalar_type() != at::kFloat8_e8m0fnu || xScale->dim() != 2 ||
+                   xScale->size(0) != x.size(0) || xScale->size(1) != blocksOf(k) || xScale->device() != x.device()
+             : x.scalar_type() != at::kBFloat16) return py::none();
+  if (at::GradMode::is_enabled() && x.requires_grad()) return py::none();
   Below below;
   c10::cuda::CUDAGuard guard(x.device());
   Tensor rows = alignedRows(x), w = whole(wIn), ws = scaleRows(wScale);
@@ -75,7 +89,7 @@ Tensor fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const Tenso
     counters().gemm += M > 0;
   }
   counters().gemm += M > 0;
-  return y;
+  return py::cast(y);
 }
 
 }  // namespace

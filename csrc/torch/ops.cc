@@ -108,40 +108,54 @@ struct PolicyLossFn : torch::autograd::Function<PolicyLossFn> {
     c10::cuda::CUDAGuard guard(logits.device());
     const int64_t rows = logits.size(0);
     auto f32 = logits.options().dtype(at::kFloat);
-    Tensor logp = at::empty({rows}, f32), stats = at::empty({3 * rows + 1}, f32), loss = at::empty({}, f32);
-    Tensor term = at::empty({rows}, f32.dtype(at::kDouble));
-    float* inverse = stats.data_ptr<float>() + 3 * rows;
+    // One buffer: the rows' terms (64 bits), three numbers a row for the backward pass, one over the divisor.
+    Tensor logp = at::empty({rows}, f32), work = at::empty({5 * rows + 1}, f32), loss = at::empty({}, f32);
+    float* stats = work.data_ptr<float>() + 2 * rows;
     check(mcclPolicyLossForward(logits.data_ptr(), logitsType(logits), rows, std::max(logits.stride(0), logits.size(1)), (int)o.vocab,
                                 tokens.data_ptr<int64_t>(), old.data_ptr<float>(), ref ? ref->data_ptr<float>() : nullptr, advantages.data_ptr<float>(),
                                 weights ? weights->data_ptr() : nullptr, weights && weights->scalar_type() == at::kBool, o.clipLow, o.clipHigh, o.klCoef,
-                                o.mean, logp.data_ptr<float>(), term.data_ptr<double>(), stats.data_ptr<float>(), loss.data_ptr<float>(), inverse,
+                                o.mean, logp.data_ptr<float>(), static_cast<double*>(work.data_ptr()), stats, loss.data_ptr<float>(), stats + 3 * rows,
                                 streamOf(logits)), "mcclPolicyLossForward");
     counters().loss += rows > 0 ? 2 : 1;
-    ctx->save_for_backward({logits, tokens, stats});
+    ctx->save_for_backward({logits, tokens, work});
     ctx->saved_data["vocab"] = o.vocab;
     ctx->mark_non_differentiable({logp});
     return {loss, logp};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2];
+    const Tensor &logits = saved[0], &tokens = saved[1];
     Below below;
     c10::cuda::CUDAGuard guard(logits.device());
     const int64_t rows = logits.size(0), width = logits.size(1);
-    Tensor go = g[0].to(at::kFloat), grad = at::empty({rows, width}, logits.options());
+    const float* stats = saved[2].data_ptr<float>() + 2 * rows;
+    Tensor go = g[0].scalar_type() == at::kFloat ? g[0] : g[0].to(at::kFloat), grad = at::empty({rows, width}, logits.options());
     check(mcclPolicyLossBackward(logits.data_ptr(), logitsType(logits), rows, std::max(logits.stride(0), width), grad.data_ptr(), width,
-                                 (int)ctx->saved_data["vocab"].toInt(), (int)width, tokens.data_ptr<int64_t>(), stats.data_ptr<float>(),
-                                 go.data_ptr<float>(), stats.data_ptr<float>() + 3 * rows, streamOf(logits)), "mcclPolicyLossBackward");
+                                 (int)ctx->saved_data["vocab"].toInt(), (int)width, tokens.data_ptr<int64_t>(), stats, go.data_ptr<float>(),
+                                 stats + 3 * rows, streamOf(logits)), "mcclPolicyLossBackward");
     counters().loss += rows > 0;
     return once({grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
-// (loss, logp).  The caller has checked types, shapes and devices.
+// (loss, logp); None where an argument is not what the kernels take (the caller says which).  vocab: all columns where missing.
 py::object policyLoss(const Tensor& logits, const Tensor& tokens, const Tensor& old, const Tensor& advantages, const std::optional<Tensor>& ref,
-                      const std::optional<Tensor>& weights, double clipLow, double clipHigh, double klCoef, int64_t vocab, bool mean) {
-  TORCH_CHECK(!recorded() && ordinary(logits), "fused_policy_loss: not under tracing, a dispatch mode or torch.func");
-  variable_list r = PolicyLossFn::apply(logits, tokens, old, advantages, ref, weights, PolicyOptions{clipLow, clipHigh, klCoef, vocab, mean});
+                      const std::optional<Tensor>& weights, double clipLow, double clipHigh, double klCoef, std::optional<int64_t> vocab, bool mean) {
+  if (recorded() || !ordinary(logits) || !logits.is_cuda() || logits.dim() != 2 || logits.size(1) == 0 || logits.size(0) > INT32_MAX ||
+      logits.size(1) > INT32_MAX - 65536) return py::none();
+  const auto type = logits.scalar_type();
+  const int64_t rows = logits.size(0), columns = vocab ? *vocab : logits.size(1);
+  auto perRow = [&](const Tensor& t, bool kind) {
+    return kind && ordinary(t) && t.dim() == 1 && t.size(0) == rows && t.device() == logits.device() && !t.requires_grad();
+  };
+  auto f32 = [&](const Tensor& t) { return perRow(t, t.scalar_type() == at::kFloat); };
+  if ((type != at::kBFloat16 && type != at::kHalf && type != at::kFloat) || !(clipLow >= 0) || !(clipHigh >= 0) || columns <= 0 || columns > logits.size(1) ||
+      (klCoef != 0 && !ref) || !perRow(tokens, tokens.scalar_type() == at::kLong) || !f32(old) || !f32(advantages) || (ref && !f32(*ref)) ||
+      (weights && !perRow(*weights, weights->scalar_type() == at::kFloat || weights->scalar_type() == at::kBool))) return py::none();
+  const bool fits = logits.stride(1) == 1 && (rows <= 1 || logits.stride(0) >= logits.size(1));
+  auto whole1d = [](const std::optional<Tensor>& t) { return t ? std::optional<Tensor>(t->contiguous()) : t; };
+  variable_list r = PolicyLossFn::apply(fits ? logits : logits.contiguous(), tokens.contiguous(), old.contiguous(), advantages.contiguous(),
+                                        whole1d(klCoef != 0 ? ref : std::nullopt), whole1d(weights), PolicyOptions{clipLow, clipHigh, klCoef, columns, mean});
   return py::make_tuple(r[0], r[1]);
 }
 
@@ -201,16 +215,20 @@ py::object gemm(const Tensor& x, const Tensor& w, const std::optional<Tensor>& o
 }
 
 // ---- products of ragged groups of rows ----------------------------------------------------------------------------------
+Tensor groupedForward(const Tensor& x, const Tensor& w, const Tensor& ends) {
+  const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1);
+  Tensor y = at::empty({T, N}, x.options());
+  check(mcclGroupedGemm(x.data_ptr(), pitchOf(x), w.data_ptr(), y.data_ptr(), ends.data_ptr(), ends.scalar_type() == at::kLong, (int)E, T, (int)N, (int)K,
+                        streamOf(x)), "mcclGroupedGemm");
+  counters().gemm += T > 0;
+  return y;
+}
+
 struct GroupedFn : torch::autograd::Function<GroupedFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& xIn, const Tensor& wIn, const Tensor& ends) {
     Below below;
     c10::cuda::CUDAGuard guard(xIn.device());
-    Tensor x = alignedRows(xIn), w = whole(wIn);
-    const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1);
-    Tensor y = at::empty({T, N}, x.options());
-    check(mcclGroupedGemm(x.data_ptr(), pitchOf(x), w.data_ptr(), y.data_ptr(), ends.data_ptr(), ends.scalar_type() == at::kLong, (int)E, T, (int)N, (int)K,
-                          streamOf(x)), "mcclGroupedGemm");
-    counters().gemm += T > 0;
+    Tensor x = alignedRows(xIn), w = whole(wIn), y = groupedForward(x, w, ends);
     ctx->save_for_backward({x, w, ends});
     return y;
   }
@@ -239,10 +257,18 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
   }
 };
 
-// The caller has checked types, shapes and devices.
-Tensor groupedGemm(const Tensor& x, const Tensor& w, const Tensor& ends) {
-  TORCH_CHECK(!recorded() && ordinary(x) && ordinary(w) && ordinary(ends), "grouped_gemm: not under tracing, a dispatch mode or torch.func");
-  return GroupedFn::apply(x, w, ends);
+// None where an argument is not what the kernels take (the caller says which).
+py::object groupedGemm(const Tensor& x, const Tensor& w, const Tensor& ends) {
+  constexpr int64_t kMost = INT32_MAX - 256;
+  if (recorded() || !ordinary(x) || !ordinary(w) || !ordinary(ends) || !bf16Cuda(x) || !bf16Cuda(w) || x.dim() != 2 || w.dim() != 3 || w.size(2) != x.size(1) ||
+      w.size(0) < 1 || w.size(0) > mcclGroupedGemmMaxGroups() || w.size(1) < 1 || w.size(1) % 8 || w.size(2) < 1 || w.size(2) % 8 || x.size(0) >= kMost ||
+      w.size(1) >= kMost || w.size(2) >= kMost) return py::none();
+  if ((ends.scalar_type() != at::kInt && ends.scalar_type() != at::kLong) || ends.dim() != 1 || ends.size(0) != w.size(0) || !ends.is_contiguous() ||
+      ends.device() != x.device() || w.device() != x.device()) return py::none();
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad())) return py::cast(GroupedFn::apply(x, w, ends));
+  Below below;
+  c10::cuda::CUDAGuard guard(x.device());
+  return py::cast(groupedForward(alignedRows(x), whole(w), ends));
 }
 
 // ---- SiLU MLP on one rank ---------------------------------------------------------------------------------------------

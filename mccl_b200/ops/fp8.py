@@ -58,7 +58,11 @@ def fp8_gemm(x: Union[torch.Tensor, BlockScaled], w: BlockScaled, ends: Optional
     [ends[e - 1], ends[e]) go through w[e] of [E, N, K], as in `grouped_gemm`: ends on the device, rows behind the last one zero.
     N is a multiple of 8, K of 16.  There is no gradient: an x that asks for one is refused (use torch.no_grad)."""
     data, scale = (x.data, x.scale) if isinstance(x, BlockScaled) else (x, None)
-    wd, ws = w.data, w.scale
+    wd, ws = w
+    y = _ext.load().fp8_gemm(data, scale, wd, ws, ends) if data.is_cuda else None
+    if y is not None:
+        return y
+    # Not taken by the kernels: say why.
     if ends is not None:
         check_groups("fp8_gemm", data, wd, ends)
     elif data.dim() != 2 or wd.dim() != 2 or data.shape[1] != wd.shape[1] or max(*data.shape, *wd.shape) >= 2 ** 31 - 256:
@@ -66,7 +70,7 @@ def fp8_gemm(x: Union[torch.Tensor, BlockScaled], w: BlockScaled, ends: Optional
     n, k = wd.shape[-2:]
     if n % 8 or k % 16 or n == 0 or k == 0:
         raise ValueError(f"fp8_gemm: N is a multiple of 8 and K of 16 (got {n} and {k})")
-    if wd.dtype != torch.float8_e4m3fn or ws.dtype != torch.float8_e8m0fnu or ws.shape != (*wd.shape[:-2], _blocks(n), _blocks(k)):
+    if wd.dtype != torch.float8_e4m3fn or ws.dtype != torch.float8_e8m0fnu or tuple(ws.shape) != (*wd.shape[:-2], _blocks(n), _blocks(k)):
         raise ValueError(f"fp8_gemm: weights are float8_e4m3fn with float8_e8m0fnu scales {[*wd.shape[:-2], _blocks(n), _blocks(k)]} "
                          f"(got {wd.dtype}, {ws.dtype} {list(ws.shape)})")
     if scale is None:
@@ -81,4 +85,4 @@ def fp8_gemm(x: Union[torch.Tensor, BlockScaled], w: BlockScaled, ends: Optional
         raise RuntimeError("fp8_gemm has no gradient: detach its rows or call it under torch.no_grad()")
     if not data.is_cuda:
         raise RuntimeError("fp8_gemm runs on CUDA (sm_100a) only")
-    return _ext.load().fp8_gemm(data, scale, wd, ws, ends)
+    raise RuntimeError("fp8_gemm does not run under tracing, a dispatch mode or torch.func")

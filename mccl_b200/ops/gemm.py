@@ -92,6 +92,10 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.
     device, e.g. the cumulative sum of the tokens per expert: the host never waits for it.  An end below an earlier one is read as
     that one, one outside [0, T] as the nearest.  Rows from ends[-1] on belong to no expert: they are zero in y and in x's gradient
     and no part of w's; the gradient of an expert without rows is zero."""
+    y = _ext.load().grouped_gemm(x, w, ends) if x.is_cuda else None
+    if y is not None:
+        return y
+    # Not taken by the kernels: say why.
     check_groups("grouped_gemm", x, w, ends)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise ValueError(f"grouped_gemm: bf16 rows and weights (got {x.dtype} and {w.dtype})")
@@ -99,7 +103,7 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.
         raise ValueError(f"grouped_gemm: N and K are multiples of 8, a row is a multiple of 16 bytes (got {w.shape[1]} and {w.shape[2]})")
     if not x.is_cuda:
         raise RuntimeError("grouped_gemm runs on CUDA (sm_100a) only")
-    return _ext.load().grouped_gemm(x, w, ends)
+    raise RuntimeError("grouped_gemm does not run under tracing, a dispatch mode or torch.func")
 
 
 def last_error() -> int:

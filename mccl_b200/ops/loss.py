@@ -41,11 +41,16 @@ def fused_policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torc
     NaN.  The last KL factor needs `ref_logp`.  Per row: int64 `tokens`, fp32 `old_logp`, `advantages`, `ref_logp`, and `weights`
     in fp32 or bool; they are constants and must not ask for a gradient.  Columns from `vocab` on are padding.  Differentiable in
     the logits, which stay as they are (the gradient has memory of its own); once only."""
-    if logits.dim() != 2 or logits.dtype not in _LOGITS or logits.shape[1] == 0 or logits.shape[0] >= 2 ** 31 or logits.shape[1] >= 2 ** 31 - 2 ** 16:
-        raise ValueError(f"fused_policy_loss: logits are a bf16, fp16 or fp32 matrix (got {logits.dtype} {tuple(logits.shape)})")
     if reduction not in ("mean", "sum"):
         raise ValueError(f"fused_policy_loss: reduction is 'mean' or 'sum' (got {reduction!r})")
     low, high = clip
+    if logits.is_cuda:
+        out = _ext.load().policy_loss(logits, tokens, old_logp, advantages, ref_logp, weights, low, high, kl_coef, vocab, reduction == "mean")
+        if out is not None:
+            return out
+    # Not taken by the kernels: say why.
+    if logits.dim() != 2 or logits.dtype not in _LOGITS or logits.shape[1] == 0 or logits.shape[0] >= 2 ** 31 or logits.shape[1] >= 2 ** 31 - 2 ** 16:
+        raise ValueError(f"fused_policy_loss: logits are a bf16, fp16 or fp32 matrix (got {logits.dtype} {tuple(logits.shape)})")
     if not (low >= 0 and high >= 0):
         raise ValueError(f"fused_policy_loss: clip is two numbers from zero on (got {clip})")
     vocab = logits.shape[1] if vocab is None else vocab
@@ -65,7 +70,4 @@ def fused_policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torc
             raise ValueError(f"fused_policy_loss: {name} is a constant: detach it")
     if not logits.is_cuda:
         raise RuntimeError("fused_policy_loss runs on CUDA (sm_100a) only")
-    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < logits.shape[1]):
-        logits = logits.contiguous()
-    args = [t if t is None else t.contiguous() for t in (tokens, old_logp, advantages, ref_logp if kl_coef != 0 else None, weights)]
-    return _ext.load().policy_loss(logits, *args, low, high, kl_coef, vocab, reduction == "mean")
+    raise RuntimeError("fused_policy_loss does not run under tracing, a dispatch mode or torch.func")
