@@ -158,6 +158,15 @@ __device__ __forceinline__ void storeTile(const uint32_t* v, uint8_t* stage, __n
     }
   }
 }
+// Zeros in a warp's 32 rows x COLS columns.
+template <int COLS>
+__device__ __forceinline__ void clearTile(__nv_bfloat16* out, int rows, int col0, int width, int lane) {
+  constexpr int PER = COLS / 8;                            // lanes a row
+  const int col = col0 + lane % PER * 8;
+#pragma unroll 4
+  for (int r = lane / PER; r < 32; r += 32 / PER)
+    if (r < rows && col < width) *reinterpret_cast<uint4*>(out + (size_t)r * width + col) = make_uint4(0, 0, 0, 0);
+}
 // The epilogue warps' share of the rows behind the last group, which belong to nobody.
 __device__ __forceinline__ void clearRows(__nv_bfloat16* out, int from, int to, int width) {
   const int64_t lo = (int64_t)from * width / 8, hi = (int64_t)to * width / 8;
@@ -260,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       Tile tile;
       const int blocks = at(t, &e, &tile);
       if (blocks == 0) continue;                           // an expert without rows: the epilogue writes zeros by itself
-      const int tail = MODE == WEIGHT ? (g.start[tile.e + 1] - g.start[tile.e]) % CK : 0;
+      const int tail = MODE == WEIGHT ? (g.start[tile.e + 1] - g.start[tile.e]) % CK : 0, steps = (tail + 15) / 16;
       if (!waitWarp<false>(&tmemEmpty[acc], accPhase ^ 1, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 32); break; }
       umma::tcFenceAfter();
       const uint32_t d = tmemBase + (uint32_t)acc * 256u;
@@ -269,9 +278,11 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
         ok = umma::mbarWait(&full[stage], phase, budget);
         if (!ok) break;
         uint8_t *pa = sA + stage * S::A_BYTES, *pb = sB + stage * S::B_BYTES;
-        if (MODE == WEIGHT && tail != 0 && kb == blocks - 1) {
-          // Rows [tail, 64) of every chunk: whole 128-byte lines, which the swizzle does not mix.
-          for (int i = lane; i < (CK - tail) * 8; i += 32) {
+        const bool behind = MODE == WEIGHT && tail != 0 && kb == blocks - 1;
+        if (behind) {
+          // MMAs of 16 rows up to the end; of the last one's, the rows behind it in every chunk: whole 128-byte lines, which the swizzle
+          // does not mix.
+          for (int i = lane; i < (steps * 16 - tail) * 8; i += 32) {
             const int off = tail * 128 + i * 16;
 #pragma unroll
             for (int c = 0; c < BM / 64; ++c) *reinterpret_cast<uint4*>(pa + c * 8192 + off) = make_uint4(0, 0, 0, 0);
@@ -285,9 +296,9 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
         if (issues) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));
           umma::mmaBf16Split(d, aLo, aHi, bLo, bHi, idesc, kb != 0);
-          umma::mmaBf16Split(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
-          umma::mmaBf16Split(d, aLo + 2 * aStep, aHi, bLo + 2 * bStep, bHi, idesc, 1);
-          umma::mmaBf16Split(d, aLo + 3 * aStep, aHi, bLo + 3 * bStep, bHi, idesc, 1);
+          if (!behind || steps > 1) umma::mmaBf16Split(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
+          if (!behind || steps > 2) umma::mmaBf16Split(d, aLo + 2 * aStep, aHi, bLo + 2 * bStep, bHi, idesc, 1);
+          if (!behind || steps > 3) umma::mmaBf16Split(d, aLo + 3 * aStep, aHi, bLo + 3 * bStep, bHi, idesc, 1);
           umma::mmaCommit(&empty[stage]);
         }
         if (++stage == ST) { stage = 0; phase ^= 1; }
@@ -304,26 +315,26 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
     for (int t = blockIdx.x; t < totalTiles; t += gridDim.x) {
       Tile tile;
       const int blocks = at(t, &e, &tile);
-      uint32_t v[COLS];
-      if (MODE == WEIGHT && blocks == 0) {
-#pragma unroll
-        for (int i = 0; i < COLS; ++i) v[i] = 0;
-      } else {
-        if (!waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 34); break; }
-        umma::tcFenceAfter();
-        const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * 256u + (uint32_t)(half * COLS);
-#pragma unroll
-        for (int c = 0; c < COLS / 32; ++c) umma::tmemLoad32x32(from + c * 32u, v + c * 32);
-        umma::tmemLoadWait();
-        umma::tcFenceBefore();
-        __syncwarp();
-        if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
-        acc ^= 1; if (acc == 0) accPhase ^= 1;
-      }
       const int r = tile.row + q * 32;
       const int limit = MODE == WEIGHT ? a.tileRows : g.start[tile.e + 1] - g.start[tile.e];
       const size_t row = MODE == WEIGHT ? (size_t)tile.e * a.tileRows + r : (size_t)g.start[tile.e] + r;
-      storeTile<COLS>(v, sStage + (warp - 4) * kStageBytes, a.out + row * (size_t)a.width, limit - r, tile.col + half * COLS, a.width, lane);
+      __nv_bfloat16* out = a.out + row * (size_t)a.width;
+      if (MODE == WEIGHT && blocks == 0) {                 // an expert without rows
+        clearTile<COLS>(out, limit - r, tile.col + half * COLS, a.width, lane);
+        continue;
+      }
+      if (!waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 34); break; }
+      umma::tcFenceAfter();
+      uint32_t v[COLS];
+      const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * 256u + (uint32_t)(half * COLS);
+#pragma unroll
+      for (int c = 0; c < COLS / 32; ++c) umma::tmemLoad32x32(from + c * 32u, v + c * 32);
+      umma::tmemLoadWait();
+      umma::tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
+      acc ^= 1; if (acc == 0) accPhase ^= 1;
+      storeTile<COLS>(v, sStage + (warp - 4) * kStageBytes, out, limit - r, tile.col + half * COLS, a.width, lane);
     }
     if (MODE != WEIGHT) clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }

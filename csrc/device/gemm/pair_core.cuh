@@ -160,14 +160,15 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
       Tile tile;
       const int blocks = at(t, &e, &tile);
       if (blocks == 0) continue;                           // an expert without rows: the epilogues write zeros by themselves
-      const bool tail = MODE == WEIGHT && (g.start[tile.e + 1] - g.start[tile.e]) % CK != 0;
+      const int tail = MODE == WEIGHT ? (g.start[tile.e + 1] - g.start[tile.e]) % CK : 0, steps = (tail + 15) / 16;
       if (!waitWarpCluster(&tmemEmpty[acc], accPhase ^ 1, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 62); break; }
       umma::tcFenceAfter();
       const uint32_t d = tmemBase + (uint32_t)(acc * BN);
       bool ok = true;
       for (int kb = 0; kb < blocks && ok; ++kb) {
         ok = umma::mbarWait(&full[stage], phase, budget);
-        if (MODE == WEIGHT && tail && kb == blocks - 1) {
+        const bool behind = MODE == WEIGHT && tail != 0 && kb == blocks - 1;
+        if (behind) {
           ok = thin::waitCluster(&tailReady[stage], tailPhase >> stage & 1, budget) && ok;
           tailPhase ^= 1u << stage;
         }
@@ -175,9 +176,9 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
         if (issues) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (B_BYTES >> 4));
           mmaBf16(d, aLo, aHi, bLo, bHi, idesc, kb != 0);
-          mmaBf16(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
-          mmaBf16(d, aLo + 2 * aStep, aHi, bLo + 2 * bStep, bHi, idesc, 1);
-          mmaBf16(d, aLo + 3 * aStep, aHi, bLo + 3 * bStep, bHi, idesc, 1);
+          if (!behind || steps > 1) mmaBf16(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
+          if (!behind || steps > 2) mmaBf16(d, aLo + 2 * aStep, aHi, bLo + 2 * bStep, bHi, idesc, 1);
+          if (!behind || steps > 3) mmaBf16(d, aLo + 3 * aStep, aHi, bLo + 3 * bStep, bHi, idesc, 1);
           commitBoth(&empty[stage]);
         }
         if (++stage == ST) { stage = 0; phase ^= 1; }
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
       acc ^= 1; if (acc == 0) accPhase ^= 1;
     }
   } else if (warp == 3 && MODE == WEIGHT) {
-    // ---------------- rows [tail, 64) of every chunk of a group's last block: whole 128-byte lines, which the swizzle does not mix
+    // ---------------- of a group's last block, the rows behind its end that the last MMA of 16 takes in (as in grouped_core.cuh)
     int stage = 0, e = 0; uint32_t tailPhase = 0;          // a bit per stage
     for (int t = pairIdx; t < totalTiles; t += pairs) {
       Tile tile;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
       if (!grouped::waitWarp<true>(&tailFull[last], tailPhase >> last & 1, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 64); break; }
       tailPhase ^= 1u << last;
       uint8_t *pa = sA + last * A_BYTES, *pb = sB + last * B_BYTES;
-      for (int i = lane; i < (CK - tail) * 8; i += 32) {
+      for (int i = lane; i < ((tail + 15) / 16 * 16 - tail) * 8; i += 32) {
         const int off = tail * 128 + i * 16;
 #pragma unroll
         for (int c = 0; c < BM / 64; ++c) *reinterpret_cast<uint4*>(pa + c * 8192 + off) = make_uint4(0, 0, 0, 0);
@@ -221,22 +222,21 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
       const int limit = MODE == WEIGHT ? a.tileRows : g.start[tile.e + 1] - g.start[tile.e];
       const size_t row = MODE == WEIGHT ? (size_t)tile.e * a.tileRows + r : (size_t)g.start[tile.e] + r;
       __nv_bfloat16* out = a.out + row * (size_t)a.width;
-      uint32_t v[HALF];
-      if (MODE == WEIGHT && blocks == 0) {
-#pragma unroll
-        for (int i = 0; i < HALF; ++i) v[i] = 0;
-      } else {
-        if (!grouped::waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 66); break; }
-        umma::tcFenceAfter();
-        const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * HALF);
-#pragma unroll
-        for (int c = 0; c < HALF / 32; ++c) umma::tmemLoad32x32(from + c * 32u, v + c * 32);
-        umma::tmemLoadWait();
-        umma::tcFenceBefore();
-        __syncwarp();
-        if (lane == 0) thin::arriveCluster(&tmemEmpty[acc], 0);
-        acc ^= 1; if (acc == 0) accPhase ^= 1;
+      if (MODE == WEIGHT && blocks == 0) {                 // an expert without rows
+        grouped::clearTile<HALF>(out, limit - r, tile.col + half * HALF, a.width, lane);
+        continue;
       }
+      if (!grouped::waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 66); break; }
+      umma::tcFenceAfter();
+      uint32_t v[HALF];
+      const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * HALF);
+#pragma unroll
+      for (int c = 0; c < HALF / 32; ++c) umma::tmemLoad32x32(from + c * 32u, v + c * 32);
+      umma::tmemLoadWait();
+      umma::tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) thin::arriveCluster(&tmemEmpty[acc], 0);
+      acc ^= 1; if (acc == 0) accPhase ^= 1;
       grouped::storeTile<HALF>(v, stage, out, limit - r, tile.col + half * HALF, a.width, lane);
     }
     if (MODE != WEIGHT) grouped::clearRows(a.out, g.start[a.groups], a.rows, a.width);

@@ -72,6 +72,9 @@ __device__ __forceinline__ void tmemLoad32x16(uint32_t taddr, uint32_t* v) {
       : "r"(taddr) : "memory");
 }
 using fp8::waitForPredecessor;
+// The two halves of a barrier over all threads of the cluster.
+__device__ __forceinline__ void clusterArrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void clusterWait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 template <int BT, bool FP8>
 __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant__ Args a) {
@@ -140,24 +143,25 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
     waitForPredecessor();
     return;
   }
-  if (warp == 2) { umma::tmemAlloc(tmemSlot, S::TMEM); umma::tmemRelinquish(); }
-  umma::tcFenceBefore();
-  __syncthreads();
-  gemm::umma2::clusterSync();                              // every rank's barriers exist before anything arrives on them
-  umma::tcFenceAfter();
-  const uint32_t tmemBase = *tmemSlot;
   const int kBlocks = (a.K + CK - 1) / CK, units = (kBlocks + UNIT - 1) / UNIT;
   const int kb0 = rank * units / slices * UNIT, kb1 = min((rank + 1) * units / slices * UNIT, kBlocks);
   const int64_t step = (int64_t)gridDim.z * BT, r0 = (int64_t)blockIdx.z * BT;
-
-  if (warp == 0 && lane == 0) {
-    // ---------------- TMA producer
-    int stage = 0; uint32_t phase = 0;
-    const int early = min(ST, kb1 - kb0);                  // weights that need not wait for the rows
+  const int early = min(ST, kb1 - kb0);                    // weights that wait for nothing
+  if (threadIdx.x == 0)
     for (int i = 0; i < early; ++i) {
       umma::mbarExpectTx(&full[i], S::A_BYTES + S::B_BYTES);
       grouped::tmaLoad3d(sA + i * S::A_BYTES, &a.mapW, &full[i], (kb0 + i) * CK, n0, e);
     }
+  if (warp == 2) { umma::tmemAlloc(tmemSlot, S::TMEM); umma::tmemRelinquish(); }
+  umma::tcFenceBefore();
+  __syncthreads();
+  umma::tcFenceAfter();
+  clusterArrive();                                         // this rank's barriers exist; the warps that reach for another's wait for its word
+  const uint32_t tmemBase = *tmemSlot;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer
+    int stage = 0; uint32_t phase = 0;
     waitForPredecessor();
     for (int64_t r = r0; r < count && *sFail == 0; r += step) {
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -251,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
     // ---------------- sums: lane quarter q holds 32 of the weights' rows, a column a row of x
     const int q = warp & 3, et = threadIdx.x - 128;
     uint32_t parity = 0;
+    clusterWait();
     for (int64_t r = r0; r < count; r += step, parity ^= 1) {
       bool ok = grouped::waitWarp<true>(tmemFull, parity, budget, sFail);
       if (!ok && lane == 0) atomicExch(a.errFlag, 56);
@@ -294,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
     }
   }
 
+  if (warp < 4) clusterWait();
   waitForPredecessor();                                    // this grid's end stands for its predecessor's too
   umma::tcFenceBefore();
   __syncthreads();
