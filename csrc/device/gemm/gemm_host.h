@@ -47,6 +47,7 @@ struct PairCall {
   int ends64, groups;
   int64_t rows;
   int N, K;
+  bool beside;                          // may run beside the product launched last on the stream
 };
 // Whether groups of this many rows are better served by pairs.
 bool pairWanted(int mode, int64_t rows, int groups, int N, int K);

@@ -55,6 +55,12 @@ template <int BN> struct Smem {
   static constexpr int TOTAL = TILE_BYTES + kEpiWarps * kStageBytes + TABLE_BYTES + 256 + 1024;
 };
 
+// The two products of a backward pass read the same dy and need nothing of each other: the second is launched with programmatic stream
+// serialization, so that its CTAs start on the SMs that the first one's last wave leaves free.  It waits for the first one's end before
+// its own, which then stands for both.
+__device__ __forceinline__ void letNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void waitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // MN-major bf16 tile written by TMA with the 128-byte swizzle: chunks of 64 columns, each 64 contracted rows of 128 bytes.
 // Leading byte offset = distance of two chunks, stride byte offset = distance of two groups of eight contracted rows.
 __device__ __forceinline__ uint64_t smemDescMn(const void* tile) {
@@ -198,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
   const int colTiles = (a.width + BN - 1) / BN;
   const int wRowTiles = MODE == WEIGHT ? (a.tileRows + BM - 1) / BM : 0;
   const uint64_t budget = a.budgetNs;
+  letNextStart();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) { umma::mbarInit(&full[s], 1); umma::mbarInit(&empty[s], 1); }
@@ -339,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
     if (MODE != WEIGHT) clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }
 
+  waitForPrevious();
   umma::tcFenceBefore();
   __syncthreads();
   if (warp == 2) umma::tmemDealloc(tmemBase, gemm::kTmemCols);

@@ -43,15 +43,25 @@ int boundDevice() {
 }
 
 template <int BN, int MODE>
-mcclResult_t launchAs(const Args& a, int dev, int grid, cudaStream_t s) {
+mcclResult_t launchAs(const Args& a, int dev, int grid, bool beside, cudaStream_t s) {
   auto* kernel = groupedKernel<BN, MODE>;
   static std::atomic<uint64_t> prepared{0};                // a bit per device: the attribute stays with the function
   if (!(prepared.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BN>::TOTAL) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
     prepared.fetch_or(1ull << (dev & 63));
   }
-  kernel<<<grid, kThreads, Smem<BN>::TOTAL, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? mcclSuccess : mcclSystemError;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem<BN>::TOTAL;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
+  return mcclSuccess;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -68,7 +78,7 @@ bool validRows(const void* p, int64_t ld, int cols) { return p != nullptr && ali
 int pickColumns(int64_t rowTiles, int width, int sms) { return width > 128 && rowTiles * ((width + 255) / 256) >= sms ? 256 : 128; }
 
 template <int MODE>
-mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn) {
+mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn, bool beside = false) {
   a.errFlag = gemm::gemmErrFlag(dev);
   if (a.errFlag == nullptr) return mcclSystemError;
   a.budgetNs = 2000000000ull;
@@ -76,11 +86,33 @@ mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_
   const int64_t tiles = rowTiles * ((a.width + bn - 1) / bn);
   if (tiles > INT32_MAX) return mcclInvalidArgument;
   const int sms = gemm::gemmSmCount(), grid = (int)(tiles < sms ? tiles : sms);
-  return bn == 256 ? launchAs<256, MODE>(a, dev, grid, stream) : launchAs<128, MODE>(a, dev, grid, stream);
+  return bn == 256 ? launchAs<256, MODE>(a, dev, grid, beside, stream) : launchAs<128, MODE>(a, dev, grid, beside, stream);
 }
 
 // Row tiles of all groups: at most one beside the full ones for each group.
 int64_t rowTilesAtMost(const Shape& s) { return s.T / BM + (s.T < s.E ? s.T : s.E); }
+
+// dw; `beside`: may run beside the product launched last on the stream.
+mcclResult_t weightGradient(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dw, const void* ends, int ends64, int groups,
+                            int64_t rows, int N, int K, bool beside, mcclStream_t stream) {
+  const Shape s{ends, ends64, groups, rows, N, K};
+  if (!valid(s) || dw == nullptr || !aligned16(dw)) return mcclInvalidArgument;
+  if (rows == 0)
+    return cudaMemsetAsync(dw, 0, (size_t)groups * N * K * 2, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? mcclSuccess : mcclSystemError;
+  if (!validRows(dy, lddy, N) || !validRows(x, ldx, K)) return mcclInvalidArgument;
+  const int dev = boundDevice();
+  if (gemm::pairWanted(WEIGHT, rows, groups, N, K))
+    return gemm::pairGemm(gemm::PairCall{WEIGHT, dy, x, lddy, ldx, dw, ends, ends64, groups, rows, N, K, beside}, dev, stream);
+  Args a;
+  memset(&a, 0, sizeof(a));
+  const int64_t rt = (int64_t)groups * ((N + BM - 1) / BM);
+  const int bn = pickColumns(rt, K, gemm::gemmSmCount());
+  MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, 64));
+  MCCLCHECK(gemm::rowsMap(&a.mapB, x, 2, 0, rows, K, ldx, 64));
+  a.tileRows = N; a.width = K;
+  a.out = static_cast<__nv_bfloat16*>(dw);
+  return run<WEIGHT>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn, beside);
+}
 
 }  // namespace
 
@@ -101,7 +133,7 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
     return gemm::thinGemm(c, dev, stream);
   }
   if (gemm::pairWanted(FORWARD, rows, groups, N, K))
-    return gemm::pairGemm(gemm::PairCall{FORWARD, x, w, ldx, K, y, ends, ends64, groups, rows, N, K}, dev, stream);
+    return gemm::pairGemm(gemm::PairCall{FORWARD, x, w, ldx, K, y, ends, ends64, groups, rows, N, K, false}, dev, stream);
   Args a;
   memset(&a, 0, sizeof(a));
   const int64_t rt = rowTilesAtMost(s);
@@ -121,7 +153,7 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
   if (!validRows(dy, lddy, N) || w == nullptr || dx == nullptr || !aligned16(w) || !aligned16(dx)) return mcclInvalidArgument;
   const int dev = boundDevice();
   if (gemm::pairWanted(DATA, rows, groups, N, K))
-    return gemm::pairGemm(gemm::PairCall{DATA, dy, w, lddy, K, dx, ends, ends64, groups, rows, N, K}, dev, stream);
+    return gemm::pairGemm(gemm::PairCall{DATA, dy, w, lddy, K, dx, ends, ends64, groups, rows, N, K, false}, dev, stream);
   Args a;
   memset(&a, 0, sizeof(a));
   const int64_t rt = rowTilesAtMost(s);
@@ -135,23 +167,13 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
 
 mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dw, const void* ends, int ends64, int groups,
                                            int64_t rows, int N, int K, mcclStream_t stream) {
-  const Shape s{ends, ends64, groups, rows, N, K};
-  if (!valid(s) || dw == nullptr || !aligned16(dw)) return mcclInvalidArgument;
-  if (rows == 0)
-    return cudaMemsetAsync(dw, 0, (size_t)groups * N * K * 2, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? mcclSuccess : mcclSystemError;
-  if (!validRows(dy, lddy, N) || !validRows(x, ldx, K)) return mcclInvalidArgument;
-  const int dev = boundDevice();
-  if (gemm::pairWanted(WEIGHT, rows, groups, N, K))
-    return gemm::pairGemm(gemm::PairCall{WEIGHT, dy, x, lddy, ldx, dw, ends, ends64, groups, rows, N, K}, dev, stream);
-  Args a;
-  memset(&a, 0, sizeof(a));
-  const int64_t rt = (int64_t)groups * ((N + BM - 1) / BM);
-  const int bn = pickColumns(rt, K, gemm::gemmSmCount());
-  MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, 64));
-  MCCLCHECK(gemm::rowsMap(&a.mapB, x, 2, 0, rows, K, ldx, 64));
-  a.tileRows = N; a.width = K;
-  a.out = static_cast<__nv_bfloat16*>(dw);
-  return run<WEIGHT>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
+  return weightGradient(dy, lddy, x, ldx, dw, ends, ends64, groups, rows, N, K, false, stream);
+}
+
+mcclResult_t mcclGroupedGemmBackward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, void* dx, void* dw, const void* ends, int ends64,
+                                     int groups, int64_t rows, int N, int K, mcclStream_t stream) {
+  MCCLCHECK(mcclGroupedGemmBackwardData(dy, lddy, w, dx, ends, ends64, groups, rows, N, K, stream));
+  return weightGradient(dy, lddy, x, ldx, dw, ends, ends64, groups, rows, N, K, rows > 0, stream);
 }
 
 }  // extern "C"

@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
   const int colTiles = (a.width + BN - 1) / BN;
   const int wRowTiles = MODE == WEIGHT ? (a.tileRows + kRows - 1) / kRows : 0;
   const uint64_t budget = a.budgetNs;
+  grouped::letNextStart();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) { umma::mbarInit(&full[s], 1); umma::mbarInit(&empty[s], 1); umma::mbarInit(&tailFull[s], 1); umma::mbarInit(&tailReady[s], 2); }
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
     if (MODE != WEIGHT) grouped::clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }
 
+  grouped::waitForPrevious();
   umma::tcFenceBefore();
   __syncthreads();
   gemm::umma2::clusterSync();                              // neither CTA frees tensor memory the other still uses

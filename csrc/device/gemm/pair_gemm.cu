@@ -16,7 +16,7 @@ using namespace mccl::pair;
 namespace {
 
 template <int MODE>
-mcclResult_t launchAs(const Args& a, int dev, int pairs, cudaStream_t s) {
+mcclResult_t launchAs(const Args& a, int dev, int pairs, bool beside, cudaStream_t s) {
   auto* kernel = pairKernel<MODE>;
   static std::atomic<uint64_t> prepared{0};                // a bit per device: the attribute stays with the function
   if (!(prepared.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
@@ -28,11 +28,13 @@ mcclResult_t launchAs(const Args& a, int dev, int pairs, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
   return mcclSuccess;
 }
@@ -72,5 +74,5 @@ mcclResult_t mccl::gemm::pairGemm(const PairCall& c, int device, void* stream) {
   a.budgetNs = 2000000000ull;
   const int grid = (int)std::min<int64_t>(tiles, pairs);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.mode == FORWARD ? launchAs<FORWARD>(a, device, grid, s) : c.mode == DATA ? launchAs<DATA>(a, device, grid, s) : launchAs<WEIGHT>(a, device, grid, s);
+  return c.mode == FORWARD ? launchAs<FORWARD>(a, device, grid, false, s) : c.mode == DATA ? launchAs<DATA>(a, device, grid, false, s) : launchAs<WEIGHT>(a, device, grid, c.beside, s);
 }

@@ -241,18 +241,20 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
     Tensor dy = alignedRows(g[0]);
     const bool wide = ends.scalar_type() == at::kLong;
     variable_list ret(3);
-    if (ctx->needs_input_grad(0)) {
-      ret[0] = at::empty({T, K}, x.options());
+    const bool data = ctx->needs_input_grad(0), weight = ctx->needs_input_grad(1);
+    if (data) ret[0] = at::empty({T, K}, x.options());
+    if (weight) ret[1] = at::empty({E, N, K}, w.options());
+    if (data && weight) {
+      check(mcclGroupedGemmBackward(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), w.data_ptr(), ret[0].data_ptr(), ret[1].data_ptr(), ends.data_ptr(),
+                                    wide, (int)E, T, (int)N, (int)K, streamOf(x)), "mcclGroupedGemmBackward");
+    } else if (data) {
       check(mcclGroupedGemmBackwardData(dy.data_ptr(), pitchOf(dy), w.data_ptr(), ret[0].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N, (int)K,
                                         streamOf(x)), "mcclGroupedGemmBackwardData");
-      counters().gemm += T > 0;
-    }
-    if (ctx->needs_input_grad(1)) {
-      ret[1] = at::empty({E, N, K}, w.options());
+    } else if (weight) {
       check(mcclGroupedGemmBackwardWeight(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), ret[1].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N,
                                           (int)K, streamOf(x)), "mcclGroupedGemmBackwardWeight");
-      counters().gemm += T > 0;
     }
+    counters().gemm += T > 0 ? data + weight : 0;
     return once(std::move(ret));
   }
 };

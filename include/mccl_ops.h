@@ -38,6 +38,9 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
                                          int64_t rows, int N, int K, mcclStream_t stream);
 mcclResult_t mcclGroupedGemmBackwardWeight(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dw, const void* ends, int ends64,
                                            int groups, int64_t rows, int N, int K, mcclStream_t stream);
+/* Both gradients; the second product starts where the first leaves SMs free. */
+mcclResult_t mcclGroupedGemmBackward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, void* dx, void* dw, const void* ends,
+                                     int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream);
 
 /* ---- 8-bit products: e4m3 values, a power-of-two scale (e8m0: its exponent + 127) for each block of 128 of a row ------------- */
 /* y [rows, N] (bf16) = x w^T with the scales of x, [rows] x [K / 128] and ldxScale bytes a row, and of w [groups, N, K], one for 128 x 128,
