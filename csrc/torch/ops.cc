@@ -108,14 +108,12 @@ struct PolicyLossFn : torch::autograd::Function<PolicyLossFn> {
     c10::cuda::CUDAGuard guard(logits.device());
     const int64_t rows = logits.size(0);
     auto f32 = logits.options().dtype(at::kFloat);
-    // One buffer: the rows' terms (64 bits), three numbers a row for the backward pass, one over the divisor.
-    Tensor logp = at::empty({rows}, f32), work = at::empty({5 * rows + 1}, f32), loss = at::empty({}, f32);
-    float* stats = work.data_ptr<float>() + 2 * rows;
+    Tensor logp = at::empty({rows}, f32), work = at::empty({3 * rows + 1}, f32), loss = at::empty({}, f32);
+    float* stats = work.data_ptr<float>();
     check(mcclPolicyLossForward(logits.data_ptr(), logitsType(logits), rows, std::max(logits.stride(0), logits.size(1)), (int)o.vocab,
                                 tokens.data_ptr<int64_t>(), old.data_ptr<float>(), ref ? ref->data_ptr<float>() : nullptr, advantages.data_ptr<float>(),
                                 weights ? weights->data_ptr() : nullptr, weights && weights->scalar_type() == at::kBool, o.clipLow, o.clipHigh, o.klCoef,
-                                o.mean, logp.data_ptr<float>(), static_cast<double*>(work.data_ptr()), stats, loss.data_ptr<float>(), stats + 3 * rows,
-                                streamOf(logits)), "mcclPolicyLossForward");
+                                o.mean, logp.data_ptr<float>(), stats, loss.data_ptr<float>(), stats + 3 * rows, streamOf(logits)), "mcclPolicyLossForward");
     counters().loss += rows > 0 ? 2 : 1;
     ctx->save_for_backward({logits, tokens, work});
     ctx->saved_data["vocab"] = o.vocab;
@@ -128,7 +126,7 @@ struct PolicyLossFn : torch::autograd::Function<PolicyLossFn> {
     Below below;
     c10::cuda::CUDAGuard guard(logits.device());
     const int64_t rows = logits.size(0), width = logits.size(1);
-    const float* stats = saved[2].data_ptr<float>() + 2 * rows;
+    const float* stats = saved[2].data_ptr<float>();
     Tensor go = g[0].scalar_type() == at::kFloat ? g[0] : g[0].to(at::kFloat), grad = at::empty({rows, width}, logits.options());
     check(mcclPolicyLossBackward(logits.data_ptr(), logitsType(logits), rows, std::max(logits.stride(0), width), grad.data_ptr(), width,
                                  (int)ctx->saved_data["vocab"].toInt(), (int)width, tokens.data_ptr<int64_t>(), stats, go.data_ptr<float>(),

@@ -157,12 +157,12 @@ mcclResult_t mcclCrossEntropyBackward(void* logits, int64_t rows, int64_t ld, in
 /* Clipped policy loss with a KL term over logits [rows, ld] (bfloat16, float16 or float32; columns from vocab on take no part):
  *   lp = z[token] - logsumexp(z), r = exp(lp - old), l = -min(r A, clamp(r, 1 - low, 1 + high) A) + kl (exp(ref - lp) - (ref - lp) - 1),
  * *loss = sum of w l, with `mean` divided by the sum of w (zero where that is zero).  logp[row] = lp.  refLogp (nullable: no KL term);
- * weights (nullable: ones): floats, or bytes of truth values.  term: rows doubles, stats: 3 x rows floats of work memory, the latter
- * and *inverse kept for the backward pass, which writes grad [rows, gradLd] (zeros from vocab to width). */
+ * weights (nullable: ones): floats, or bytes of truth values.  stats: 3 x rows floats of work memory, kept with *inverse for the
+ * backward pass, which writes grad [rows, gradLd] (zeros from vocab to width). */
 mcclResult_t mcclPolicyLossForward(const void* logits, mcclDataType_t dt, int64_t rows, int64_t ld, int vocab, const int64_t* tokens,
                                    const float* oldLogp, const float* refLogp, const float* advantages, const void* weights, int boolWeights,
-                                   double clipLow, double clipHigh, double klCoef, int mean, float* logp, double* term, float* stats, float* loss,
-                                   float* inverse, mcclStream_t stream);
+                                   double clipLow, double clipHigh, double klCoef, int mean, float* logp, float* stats, float* loss, float* inverse,
+                                   mcclStream_t stream);
 mcclResult_t mcclPolicyLossBackward(const void* logits, mcclDataType_t dt, int64_t rows, int64_t ld, void* grad, int64_t gradLd, int vocab,
                                     int width, const int64_t* tokens, const float* stats, const float* gradOut, const float* inverse,
                                     mcclStream_t stream);
