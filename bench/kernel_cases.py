@@ -6,6 +6,9 @@ L2, a few hundred MB on the device, a handful of launches) and for quick CUDA-ev
     python bench/kernel_cases.py adamw  [--elems 67108864]
     python bench/kernel_cases.py sumsq  [--elems 268435456]
     python bench/kernel_cases.py copy   [--mbytes 512]      (staging copy kernel through a 1-rank communicator)
+    python bench/kernel_cases.py grouped [--m 8192 --n 2048 --k 1024 --experts 8]   (ragged products, forward and both gradients)
+    python bench/kernel_cases.py fp8    [--m 8192 --n 3584 --k 8192]     (8-bit product of quantised rows, and with their quantisation)
+    python bench/kernel_cases.py policy [--m 8192 --n 50257]             (policy loss over m x n bf16 logits, forward and with the gradient)
     python bench/kernel_cases.py emu    [--ranks 8 --mbytes 64 --algo twoshot|oneshot|ring|tree]
                                         (multi-rank all-reduce kernels with the ranks emulated on this one GPU)
 
@@ -51,12 +54,13 @@ def timed(fn, launches, warm=2):
 
 def main() -> int:
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["gemm", "adamw", "sumsq", "copy", "emu"])
+    ap.add_argument("case", choices=["gemm", "grouped", "fp8", "policy", "adamw", "sumsq", "copy", "emu"])
     ap.add_argument("--ranks", type=int, default=8)
     ap.add_argument("--algo", default="twoshot")
     ap.add_argument("--m", type=int, default=8192)
     ap.add_argument("--n", type=int, default=3584)
     ap.add_argument("--k", type=int, default=8192)
+    ap.add_argument("--experts", type=int, default=8)
     ap.add_argument("--elems", type=int, default=0)
     ap.add_argument("--mbytes", type=int, default=512)
     ap.add_argument("--launches", type=int, default=3)
@@ -81,6 +85,41 @@ def main() -> int:
             ref_ms = timed(lambda: torch.matmul(x, w.t(), out=y), args.launches)
             out.update({"cublas_us": round(ref_ms * 1e3, 1), "cublas_tflops": round(fl / ref_ms / 1e9, 1),
                         "speedup_vs_cublas": round(ref_ms / ms, 3)})
+    elif args.case == "grouped":
+        from mccl_b200.ops import gemm as G
+        t, n, k, e = args.m, args.n, args.k, args.experts
+        x = torch.randn(t, k, device=dev).to(torch.bfloat16).requires_grad_(True)
+        w = (torch.randn(e, n, k, device=dev) * k ** -0.5).to(torch.bfloat16).requires_grad_(True)
+        dy = torch.randn(t, n, device=dev).to(torch.bfloat16)
+        share = torch.rand(e, device=dev) + 0.5                     # groups of uneven sizes
+        ends = (share.cumsum(0) / share.sum() * t).round().to(torch.int32)
+        with torch.no_grad():
+            fwd = timed(lambda: G.grouped_gemm(x, w, ends), args.launches)
+        both = timed(lambda: torch.autograd.grad(G.grouped_gemm(x, w, ends), [x, w], dy), args.launches)
+        fl = 2.0 * t * n * k
+        out.update({"shape": [t, n, k], "experts": e, "forward_us": round(fwd * 1e3, 1), "forward_tflops": round(fl / fwd / 1e9, 1),
+                    "with_gradients_us": round(both * 1e3, 1), "with_gradients_tflops": round(3 * fl / both / 1e9, 1), "kernel_error": G.last_error()})
+    elif args.case == "fp8":
+        from mccl_b200.ops import fp8 as Q
+        from mccl_b200.ops import gemm as G
+        x = torch.randn(args.m, args.k, device=dev).to(torch.bfloat16)
+        w = Q.fp8_quantize((torch.randn(args.n, args.k, device=dev) * 0.02).to(torch.bfloat16), rows=128)
+        xq = Q.fp8_quantize(x)
+        ms, both = timed(lambda: Q.fp8_gemm(xq, w), args.launches), timed(lambda: Q.fp8_gemm(x, w), args.launches)
+        fl = 2.0 * args.m * args.n * args.k
+        out.update({"shape": [args.m, args.n, args.k], "us": round(ms * 1e3, 1), "tflops": round(fl / ms / 1e9, 1),
+                    "with_quantisation_us": round(both * 1e3, 1), "kernel_error": G.last_error()})
+    elif args.case == "policy":
+        from mccl_b200.ops.loss import fused_policy_loss
+        rows, vocab = args.m, args.n if args.n != 3584 else 50257
+        z = torch.randn(rows, vocab, device=dev).to(torch.bfloat16)
+        a, old, adv = torch.randint(0, vocab, (rows,), device=dev), torch.full((rows,), -11.0, device=dev), torch.randn(rows, device=dev)
+        with torch.no_grad():
+            fwd = timed(lambda: fused_policy_loss(z, a, old, adv), args.launches)
+        zr = z.requires_grad_(True)
+        both = timed(lambda: torch.autograd.grad(fused_policy_loss(zr, a, old, adv)[0], zr), args.launches)
+        out.update({"rows": rows, "vocab": vocab, "forward_us": round(fwd * 1e3, 1), "with_gradient_us": round(both * 1e3, 1),
+                    "gbs": round(6 * rows * vocab / both / 1e6, 1), "frac_of_copy_peak": round(6 * rows * vocab / both / 1e6 / hbm, 3)})
     elif args.case == "adamw":
         from mccl_b200.ops.optim import fused_adamw_
         n = args.elems or (64 << 20)

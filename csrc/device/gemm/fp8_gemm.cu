@@ -51,10 +51,11 @@ mcclResult_t product(const void* x, int64_t ldx, const void* xScale, int64_t ldx
   int dev = 0;
   cudaGetDevice(&dev);
   cudaSetDevice(dev);                                      // binds the context to this thread, for the driver's encoder
-  if (gemm::thinWanted(rows, ends != nullptr, groups, N))
+  if (gemm::thinWanted(rows, ends != nullptr, groups, N, K))
     return gemm::thinGemm(gemm::ThinCall{x, w, ldx, true, xScale, wScale, ldxScale, ldwScale, y, ends, ends64, groups, rows, N, K, behind}, dev, stream);
   const int64_t rowTiles = ends == nullptr ? (rows + BM - 1) / BM : rows / BM + (rows < groups ? rows : groups);
-  const int sms = gemm::gemmSmCount(), bn = N > 128 && rowTiles * ((N + 255) / 256) >= sms ? 256 : 128;
+  const int sms = gemm::gemmSmCount();
+  const int bn = gemm::pickColumns(ends == nullptr ? (double)rowTiles : (double)(rows / BM) + 0.5 * (double)(rows < groups ? rows : groups), N, sms);
   const int64_t tiles = rowTiles * ((N + bn - 1) / bn);
   if (tiles > INT32_MAX) return mcclInvalidArgument;
   Args a;

@@ -34,8 +34,8 @@ struct ThinCall {
   int N, K;
   bool behind;
 };
-// Whether this many rows are better served by the thin form: where the tiles of 128 rows x 128 columns are no more than the SMs.
-bool thinWanted(int64_t rows, bool ragged, int groups, int N);
+// Whether this many rows are better served by the thin form.  kBytes: of a row of the weights.
+bool thinWanted(int64_t rows, bool ragged, int groups, int N, int64_t kBytes);
 mcclResult_t thinGemm(const ThinCall& c, int device, void* stream);
 // The products of groups by pairs of SMs (pair_core.cuh).  mode: 0 y = x w^T, 1 dx = dy w, 2 dw = dy^T x.
 struct PairCall {
@@ -52,6 +52,9 @@ struct PairCall {
 // Whether groups of this many rows are better served by pairs.
 bool pairWanted(int mode, int64_t rows, int groups, int N, int K);
 mcclResult_t pairGemm(const PairCall& c, int device, void* stream);
+// Columns of a tile of 128 rows, 128 or 256, by the waves that so many row tiles of `width` columns make.  A wave of tiles of 128 columns takes 0.8 of one
+// of 256 (8 bits, contraction of 8192: 21 and 26 us), so the narrow tile is for where SMs would stand idle.
+int pickColumns(double rowTiles, int width, int sms);
 // Tensor map of [outer][rows][cols] (outer 0: a matrix) of 2-byte (bf16) or 1-byte elements, rows `ld` elements apart: boxes of 128 bytes x
 // boxRows, 128-byte swizzle, zeros outside.
 mcclResult_t rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxRows);

@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "../../core/core.h"
 #include "gemm_host.h"
@@ -12,6 +13,15 @@
 
 using namespace mccl;
 using namespace mccl::grouped;
+
+int mccl::gemm::pickColumns(double rowTiles, int width, int sms) {
+  if (width <= 128) return 128;
+  auto waves = [&](int bn) {
+    const double w = rowTiles * ((width + bn - 1) / bn) / sms;
+    return w > 8 ? w : std::ceil(w);
+  };
+  return waves(128) * 0.8 < waves(256) ? 128 : 256;
+}
 
 mcclResult_t mccl::gemm::rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld,
                                  uint32_t boxRows) {
@@ -73,10 +83,6 @@ bool valid(const Shape& s) {
 }
 bool validRows(const void* p, int64_t ld, int cols) { return p != nullptr && aligned16(p) && ld >= cols && ld % 8 == 0; }
 
-// Columns of a tile: 256 where that gives every SM a tile, else 128 (an MMA of 128 rows takes nearly as long with 128 columns as
-// with 256, so the narrow tile is worth its while only where SMs would stand idle).
-int pickColumns(int64_t rowTiles, int width, int sms) { return width > 128 && rowTiles * ((width + 255) / 256) >= sms ? 256 : 128; }
-
 template <int MODE>
 mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn, bool beside = false) {
   a.errFlag = gemm::gemmErrFlag(dev);
@@ -91,6 +97,8 @@ mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_
 
 // Row tiles of all groups: at most one beside the full ones for each group.
 int64_t rowTilesAtMost(const Shape& s) { return s.T / BM + (s.T < s.E ? s.T : s.E); }
+// and half of one on the average.
+double rowTilesExpected(const Shape& s) { return (double)(s.T / BM) + 0.5 * (double)(s.T < s.E ? s.T : s.E); }
 
 // dw; `beside`: may run beside the product launched last on the stream.
 mcclResult_t weightGradient(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dw, const void* ends, int ends64, int groups,
@@ -106,7 +114,7 @@ mcclResult_t weightGradient(const void* dy, int64_t lddy, const void* x, int64_t
   Args a;
   memset(&a, 0, sizeof(a));
   const int64_t rt = (int64_t)groups * ((N + BM - 1) / BM);
-  const int bn = pickColumns(rt, K, gemm::gemmSmCount());
+  const int bn = gemm::pickColumns((double)rt, K, gemm::gemmSmCount());
   MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, 64));
   MCCLCHECK(gemm::rowsMap(&a.mapB, x, 2, 0, rows, K, ldx, 64));
   a.tileRows = N; a.width = K;
@@ -127,7 +135,7 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
   if (rows == 0) return mcclSuccess;
   if (!validRows(x, ldx, K) || w == nullptr || y == nullptr || !aligned16(w) || !aligned16(y)) return mcclInvalidArgument;
   const int dev = boundDevice();
-  if (gemm::thinWanted(rows, true, groups, N)) {
+  if (gemm::thinWanted(rows, true, groups, N, 2ll * K)) {
     gemm::ThinCall c{};
     c.x = x; c.w = w; c.ldx = ldx; c.out = y; c.ends = ends; c.ends64 = ends64; c.groups = groups; c.rows = rows; c.N = N; c.K = K;
     return gemm::thinGemm(c, dev, stream);
@@ -137,7 +145,7 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
   Args a;
   memset(&a, 0, sizeof(a));
   const int64_t rt = rowTilesAtMost(s);
-  const int bn = pickColumns(rt, N, gemm::gemmSmCount());
+  const int bn = gemm::pickColumns(rowTilesExpected(s), N, gemm::gemmSmCount());
   MCCLCHECK(gemm::rowsMap(&a.mapA, x, 2, 0, rows, K, ldx, BM));
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, bn));
   a.contracted = K; a.width = N;
@@ -157,7 +165,7 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
   Args a;
   memset(&a, 0, sizeof(a));
   const int64_t rt = rowTilesAtMost(s);
-  const int bn = pickColumns(rt, K, gemm::gemmSmCount());
+  const int bn = gemm::pickColumns(rowTilesExpected(s), K, gemm::gemmSmCount());
   MCCLCHECK(gemm::rowsMap(&a.mapA, dy, 2, 0, rows, N, lddy, BM));
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, 64));
   a.contracted = N; a.width = K;

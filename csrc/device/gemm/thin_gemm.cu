@@ -49,13 +49,23 @@ mcclResult_t launch(int bt, Args& a, const gemm::ThinCall& c, int dev, int tiles
   }
 }
 
+// CTAs that run at a time.  Two fit an SM, but clusters do not fill the last of them: 128 rows of 8192 by 3584 columns with 280 CTAs in clusters of
+// five 19 us, with 224 in clusters of four 13 us.
+int64_t placesFor(int64_t sms) { return 2 * sms * 7 / 8; }
+
 int64_t expertsWithRows(int64_t rows, int groups) { return std::min<int64_t>(rows, groups); }
 
 }  // namespace
 
-bool mccl::gemm::thinWanted(int64_t rows, bool ragged, int groups, int N) {
-  const int64_t rowTiles = ragged ? rows / BM + expertsWithRows(rows, groups) : (rows + BM - 1) / BM;
-  return rowTiles * ((N + BM - 1) / BM) <= gemmSmCount();
+// Where a tile's contraction can be shared by two CTAs or more (8 bits, 100 rows of 8192 by 11008 columns, which cannot: 32 us here, 21 us in tiles of
+// 128 rows), and for up to 32 rows whose weights' rows are not short (one row of 4096 by 22016 columns 14.5 us here, 26 us there; of 1024 by
+// 50304 columns 14.4 and 12.9 us).  With groups, whose rows the host does not know: where the tiles of 128 rows x 128 columns are no more than
+// the SMs (64 rows for 32 experts of 2048 x 5504, which are more: 106 us here, 103 us there).
+bool mccl::gemm::thinWanted(int64_t rows, bool ragged, int groups, int N, int64_t kBytes) {
+  const int64_t nTiles = (N + BM - 1) / BM, sms = gemmSmCount();
+  if (ragged) return (rows / BM + expertsWithRows(rows, groups)) * nTiles <= sms;
+  if (rows <= 32) return nTiles <= sms || kBytes >= 2048;
+  return 2 * nTiles * ((rows + 63) / 64) <= placesFor(sms);
 }
 
 mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
@@ -65,10 +75,8 @@ mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
   const int64_t experts = ragged ? expertsWithRows(c.rows, c.groups) : 1, rows = ragged ? 2 * ((c.rows + experts - 1) / experts) : c.rows;
   const int bt = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   const int64_t shares = (rows + bt - 1) / bt;             // an expert with more rows than expected walks them in turns
-  // CTAs a tile: as many as run at a time.  Two fit an SM, but clusters do not fill the last of them: 128 rows of 8192 by 3584 columns with
-  // 280 CTAs in clusters of five 19 us, with 224 in clusters of four 13 us.
   const int perUnit = c.fp8 ? 512 : 64, units = (c.K + perUnit - 1) / perUnit;
-  const int64_t places = 2ll * sms * 7 / 8, tiles = (int64_t)nTiles * c.groups * shares;       // those of experts without rows start, too
+  const int64_t places = placesFor(sms), tiles = (int64_t)nTiles * c.groups * shares;       // those of experts without rows start, too
   const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8, places / tiles, units}));
   Args a;
   memset(&a, 0, sizeof(a));

@@ -5,7 +5,7 @@
     fsdp        FullyShardedStack: parameters, gradients and optimizer state sharded per block (ZeRO-3)
     tp          TensorParallelFFN / FusedTensorParallelMLP: the fused all-gather -> GEMM and GEMM -> reduce-scatter kernels
     functional  the collectives as differentiable functions, ring attention
-    layers      column / row parallel linear, sequence-parallel MLP, Ulysses and ring attention, expert-parallel MoE
+    layers      column / row parallel linear, sequence-parallel MLP, Ulysses and ring attention, expert-parallel and dropless MoE
     pipeline    PipelineStage: 1F1B over grouped Send / Recv
 
 Submodules are imported on demand (`from mccl_b200.parallel import layers`): `tp` needs CUDA at call time, the others

@@ -9,6 +9,8 @@
                                                                    travel around the ring of ranks
     ExpertParallelMoE                                              top-1 routed experts spread over the ranks,
                                                                    dispatch and combine by all-to-all
+    DroplessMoE                                                    top-k routed experts of one GPU, no token dropped:
+                                                                   ragged products, in 8 bits for serving
 
 They run on whatever device their tensors live on: cuda tensors use the library's kernels, cpu tensors the tcp
 transport (which is how they are tested without a GPU).  The inference-only `TensorParallelFFN` in `tp.py` is the
@@ -217,6 +219,78 @@ class ExpertParallelMoE(nn.Module):
         return y.index_put((keep.nonzero(as_tuple=True)[0],), got[flat[keep]] * gate[keep].unsqueeze(-1))
 
 
+def _by_expert(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """ops.gemm.grouped_gemm; as separate products where its kernels do not run (which read the ends on the host)."""
+    if x.dtype == w.dtype == torch.bfloat16 and not (x.shape[1] % 8 or w.shape[1] % 8) and may_fuse(x, w, ends):
+        from ..ops.gemm import grouped_gemm
+        return grouped_gemm(x, w, ends)
+    at = [0, *ends.tolist()]
+    return torch.cat([F.linear(x[a:b], w[e]) for e, (a, b) in enumerate(zip(at, at[1:]))])
+
+
+class DroplessMoE(nn.Module):
+    """Top-k routed mixture of experts with all experts on this GPU and no capacity: every token goes to the `top_k` experts with the
+    largest router probabilities and is weighted by them (divided by their sum).  The tokens are sorted by expert and the experts are
+    two products over ragged groups (ops/gemm.py), in bf16 on CUDA; nothing is padded or dropped and the host waits for nothing.
+    `quantized()` gives the layer for serving, with the experts in 8 bits."""
+
+    def __init__(self, hidden: int, ffn: int, experts: int, top_k: int = 2, device=None, dtype=None):
+        super().__init__()
+        if not 0 < top_k <= experts:
+            raise ValueError(f"top_k is 1 to the number of experts (got {top_k} of {experts})")
+        self.hidden, self.ffn, self.experts, self.top_k = hidden, ffn, experts, top_k
+        self.router = nn.Linear(hidden, experts, bias=False, device=device, dtype=dtype)
+        self.w_in = nn.Parameter(torch.empty(experts, ffn, hidden, device=device, dtype=dtype))
+        self.w_out = nn.Parameter(torch.empty(experts, hidden, ffn, device=device, dtype=dtype))
+        nn.init.normal_(self.w_in, std=hidden ** -0.5)
+        nn.init.normal_(self.w_out, std=ffn ** -0.5)
+
+    def route(self, x: torch.Tensor):
+        """Weights (in x's type) and experts [T, top_k] of every token."""
+        weight, expert = F.softmax(self.router(x).float(), dim=-1).topk(self.top_k, dim=-1)
+        return (weight / weight.sum(-1, keepdim=True)).to(x.dtype), expert
+
+    def products(self, rows: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+        """The experts' MLP on rows sorted by expert."""
+        return _by_expert(F.silu(_by_expert(rows, self.w_in, ends)), self.w_out, ends)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        t, k = x.shape[0], self.top_k
+        weight, expert = self.route(x)
+        by_expert, order = expert.reshape(-1).sort(stable=True)
+        ends = torch.searchsorted(by_expert, torch.arange(self.experts, device=x.device), right=True)
+        # Every row once in either direction: the gradients of the copies of a token are added up in the order of its experts.
+        rows = x.unsqueeze(1).expand(t, k, self.hidden).reshape(t * k, self.hidden).index_select(0, order)
+        out = self.products(rows, ends).index_select(0, order.argsort())
+        return (out.view(t, k, self.hidden) * weight.unsqueeze(-1)).sum(1)
+
+    def quantized(self) -> "QuantizedMoE":
+        """The layer for serving: its own copy of the experts as they are now, in 8 bits; the router is this one's."""
+        return QuantizedMoE(self)
+
+
+class QuantizedMoE(DroplessMoE):
+    """DroplessMoE with its experts in 8 bits with a scale for each block of 128 (ops/fp8.py), for serving: no gradients.  Made by
+    `DroplessMoE.quantized()`; hidden and ffn are multiples of 16, tokens bf16 on CUDA."""
+
+    def __init__(self, layer: DroplessMoE):
+        from ..ops.fp8 import fp8_quantize
+        nn.Module.__init__(self)
+        self.hidden, self.ffn, self.experts, self.top_k, self.router = layer.hidden, layer.ffn, layer.experts, layer.top_k, layer.router
+        self.w_in, self.w_out = fp8_quantize(layer.w_in.detach(), rows=128), fp8_quantize(layer.w_out.detach(), rows=128)
+
+    def products(self, rows: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+        from ..ops.fp8 import fp8_gemm
+        return fp8_gemm(F.silu(fp8_gemm(rows, self.w_in, ends)), self.w_out, ends)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return super().forward(x)
+
+    def quantized(self) -> "QuantizedMoE":
+        return self
+
+
 def moe_reference(x: torch.Tensor, router_w: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, capacity: int) -> torch.Tensor:
     """Dense restatement of ExpertParallelMoE for one rank's tokens: w_in / w_out hold ALL experts ([E, ffn, hidden],
     [E, hidden, ffn]); the capacity rule is applied to this rank's tokens as the layer applies it."""
@@ -230,6 +304,15 @@ def moe_reference(x: torch.Tensor, router_w: torch.Tensor, w_in: torch.Tensor, w
     return y * keep.unsqueeze(-1)
 
 
+def dropless_moe_reference(x: torch.Tensor, router_w: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, top_k: int) -> torch.Tensor:
+    """Dense restatement of DroplessMoE: every expert on every token, the others' weights zero."""
+    p = F.softmax((x @ router_w.t()).float(), dim=-1)
+    top = p.topk(top_k, dim=-1)
+    weight = torch.zeros_like(p).scatter(1, top.indices, top.values / top.values.sum(-1, keepdim=True)).to(x.dtype)
+    h = F.silu(torch.einsum("td,efd->tef", x, w_in))
+    return torch.einsum("tef,edf,te->td", h, w_out, weight)
+
+
 def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True) -> torch.Tensor:
     """[tokens, heads, d] attention on one process."""
     o = F.scaled_dot_product_attention(q.transpose(0, 1).unsqueeze(0), k.transpose(0, 1).unsqueeze(0),
@@ -238,4 +321,4 @@ def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causa
 
 
 __all__ = ["ColumnParallelLinear", "RowParallelLinear", "TensorParallelMLP", "UlyssesAttention", "RingAttention", "ExpertParallelMoE",
-           "moe_reference", "attention_reference"]
+           "DroplessMoE", "QuantizedMoE", "moe_reference", "dropless_moe_reference", "attention_reference"]
