@@ -23,7 +23,7 @@ int gemmSmCount();
 // kernel that makes x and its scales, which lets it start early.
 struct ThinCall {
   const void *x, *w;
-  int64_t ldx;                          // elements
+  int64_t ldx, ldw;                     // elements
   bool fp8;
   const void *sx, *sw;
   int64_t ldsx, ldsw;

@@ -137,7 +137,7 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
   const int dev = boundDevice();
   if (gemm::thinWanted(rows, true, groups, N, 2ll * K)) {
     gemm::ThinCall c{};
-    c.x = x; c.w = w; c.ldx = ldx; c.out = y; c.ends = ends; c.ends64 = ends64; c.groups = groups; c.rows = rows; c.N = N; c.K = K;
+    c.x = x; c.w = w; c.ldx = ldx; c.ldw = K; c.out = y; c.ends = ends; c.ends64 = ends64; c.groups = groups; c.rows = rows; c.N = N; c.K = K;
     return gemm::thinGemm(c, dev, stream);
   }
   if (gemm::pairWanted(FORWARD, rows, groups, N, K))

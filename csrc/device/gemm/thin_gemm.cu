@@ -80,7 +80,7 @@ mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
   const int slices = (int)std::max<int64_t>(1, std::min<int64_t>({8, places / tiles, units}));
   Args a;
   memset(&a, 0, sizeof(a));
-  MCCLCHECK(rowsMap(&a.mapW, c.w, c.fp8 ? 1 : 2, c.groups, c.N, c.K, c.K, BM));
+  MCCLCHECK(rowsMap(&a.mapW, c.w, c.fp8 ? 1 : 2, c.groups, c.N, c.K, c.ldw, BM));
   a.sx = static_cast<const uint8_t*>(c.sx);
   a.sw = static_cast<const uint8_t*>(c.sw);
   a.ldsx = c.ldsx; a.ldsw = c.ldsw;

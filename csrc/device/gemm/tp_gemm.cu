@@ -150,8 +150,13 @@ ErrFlag errFlagFor(int device) {
   ErrFlag& f = flags[device];
   if (f.host == nullptr) {
     int *host = nullptr, *dev = nullptr;
-    if (cudaHostAlloc((void**)&host, 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { cudaGetLastError(); return ErrFlag{}; }
-    if (cudaHostGetDevicePointer((void**)&dev, host, 0) != cudaSuccess) { cudaGetLastError(); cudaFreeHost(host); return ErrFlag{}; }
+    // The first launch of all may be one that a stream records: memory of the host is no part of the recording.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const bool ok = cudaHostAlloc((void**)&host, 64, cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess &&
+                    cudaHostGetDevicePointer((void**)&dev, host, 0) == cudaSuccess;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) { cudaGetLastError(); if (host != nullptr) cudaFreeHost(host); return ErrFlag{}; }
     *host = 0;
     f.host = host; f.dev = dev;
   }

@@ -50,8 +50,8 @@ __device__ __forceinline__ uint2 quantize(const uint4& q, uint32_t byte) {
 // I: the type the blocks of all rows are counted in (a 64-bit division costs as much as the rest).
 constexpr int kPieces = 4, kPerBlock = 8;
 template <class I>
-__global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, uint8_t* scale, int64_t lds, int64_t rows, int K,
-                                                               int blocks) {
+__global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int64_t rows,
+                                                               int K, int blocks) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // a product behind this may start; it waits for this grid's end where it reads
   const I total = (I)rows * (I)blocks, b0 = (I)blockIdx.x * (kThreads / kPerBlock * kPieces) + (threadIdx.x / kPerBlock);
   const int in = (threadIdx.x % kPerBlock) * 16;
@@ -78,20 +78,21 @@ __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat
     const int col = blk[u] * kBlock + in;
     if (blk[u] >= 0 && col < K) {
       const uint2 lo = quantize(v[u][0], byte), hi = quantize(v[u][1], byte);
-      *reinterpret_cast<uint4*>(q + row[u] * K + col) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      *reinterpret_cast<uint4*>(q + row[u] * ldq + col) = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
     if (blk[u] >= 0 && in == 0) scale[row[u] * lds + blk[u]] = (uint8_t)byte;
   }
 }
 
 // One CTA a block of 128 x 128: each thread eight rows' pieces of eight values.
-__global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloat16* x, uint8_t* q, uint8_t* scale, int64_t lds, int rows, int K, int rowBlocks) {
+__global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloat16* x, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int rows, int K,
+                                                                int rowBlocks) {
   __shared__ uint32_t warpMax[kThreads / 32];
   const int rb = (int)(blockIdx.y % rowBlocks);
   const int64_t outer = blockIdx.y / rowBlocks;
   const int col = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
   x += outer * rows * K;
-  q += outer * rows * K;
+  q += outer * rows * ldq;
   uint4 v[8];
   uint32_t a = 0;
 #pragma unroll
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloa
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = rb * kBlock + i * 16 + (threadIdx.x >> 4);
-    if (r < rows && col < K) *reinterpret_cast<uint2*>(q + (int64_t)r * K + col) = quantize(v[i], byte);
+    if (r < rows && col < K) *reinterpret_cast<uint2*>(q + r * ldq + col) = quantize(v[i], byte);
   }
   if (threadIdx.x == 0) scale[(outer * rowBlocks + rb) * lds + blockIdx.x] = (uint8_t)byte;
 }
@@ -121,20 +122,21 @@ mcclResult_t launchedOk() { return cudaGetLastError() == cudaSuccess ? mcclSucce
 
 extern "C" {
 
-mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, void* scale, int64_t ldScale, int64_t rows, int K, mcclStream_t stream) {
+mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, int64_t ldq, void* scale, int64_t ldScale, int64_t rows, int K, mcclStream_t stream) {
   const int blocks = (K + kBlock - 1) / kBlock;
-  if (rows < 0 || K <= 0 || K > INT32_MAX - 256 || K % 16 || ldx < K || ldx % 8 || ldScale < blocks) return mcclInvalidArgument;
+  if (rows < 0 || K <= 0 || K > INT32_MAX - 256 || K % 16 || ldx < K || ldx % 8 || ldq < K || ldq % 16 || ldScale < blocks) return mcclInvalidArgument;
   if (rows == 0) return mcclSuccess;
   if (!x || !q || !scale || !aligned16(x) || !aligned16(q) || rows * blocks > (int64_t)INT32_MAX * 16) return mcclInvalidArgument;
   const int64_t per = kThreads / kPerBlock * kPieces, ctas = (rows * blocks + per - 1) / per;
   auto* kernel = rows * blocks < (1ll << 31) - per ? quantizeRowsKernel<uint32_t> : quantizeRowsKernel<int64_t>;
   kernel<<<(unsigned)ctas, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q),
-                                                                                  static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
+                                                                                  ldq, static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
   return launchedOk();
 }
 
-mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, void* scale, int64_t ldScale, int64_t outer, int rows, int K, mcclStream_t stream) {
-  if (outer < 0 || rows <= 0 || K <= 0 || K > INT32_MAX - 256 || rows > INT32_MAX - 256 || K % 16 || ldScale < (K + kBlock - 1) / kBlock) return mcclInvalidArgument;
+mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, int64_t ldq, void* scale, int64_t ldScale, int64_t outer, int rows, int K, mcclStream_t stream) {
+  if (outer < 0 || rows <= 0 || K <= 0 || K > INT32_MAX - 256 || rows > INT32_MAX - 256 || K % 16 || ldq < K || ldq % 16 || ldScale < (K + kBlock - 1) / kBlock)
+    return mcclInvalidArgument;
   if (outer == 0) return mcclSuccess;
   const int rowBlocks = (rows + kBlock - 1) / kBlock;
   if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return mcclInvalidArgument;
@@ -144,8 +146,8 @@ mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, void* scale, int64_t l
   for (int64_t o = 0; o < outer; o += per) {
     const int64_t n = outer - o < per ? outer - o : per;
     quantizeTilesKernel<<<dim3((unsigned)((K + kBlock - 1) / kBlock), (unsigned)(n * rowBlocks)), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-        static_cast<const __nv_bfloat16*>(x) + o * rows * K, static_cast<uint8_t*>(q) + o * rows * K, static_cast<uint8_t*>(scale) + o * rowBlocks * ldScale,
-        ldScale, rows, K, rowBlocks);
+        static_cast<const __nv_bfloat16*>(x) + o * rows * K, static_cast<uint8_t*>(q) + o * rows * ldq, ldq,
+        static_cast<uint8_t*>(scale) + o * rowBlocks * ldScale, ldScale, rows, K, rowBlocks);
   }
   return launchedOk();
 }

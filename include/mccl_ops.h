@@ -45,17 +45,19 @@ mcclResult_t mcclGroupedGemmBackward(const void* dy, int64_t lddy, const void* x
 /* ---- 8-bit products: e4m3 values, a power-of-two scale (e8m0: its exponent + 127) for each block of 128 of a row ------------- */
 /* y [rows, N] (bf16) = x w^T with the scales of x, [rows] x [K / 128] and ldxScale bytes a row, and of w [groups, N, K], one for 128 x 128,
  * [groups][N / 128] x [K / 128] and ldwScale bytes a row (row pitches a multiple of 4, counts rounded up); fp32 sums.  ends (null: one
- * group) as in mcclGroupedGemm.  N a multiple of 8, K and ldx of 16; values 16-byte, scales 4-byte aligned. */
-mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t ldxScale, const void* w, const void* wScale, int64_t ldwScale,
-                         void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream);
-/* The same for bf16 x [rows, K] (16-byte aligned, ldx a multiple of 8), quantised into q [rows, K] and its scales first. */
-mcclResult_t mcclFp8GemmBf16Rows(const void* x, int64_t ldx, void* q, void* qScale, int64_t ldqScale, const void* w, const void* wScale,
-                                 int64_t ldwScale, void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K,
+ * group) as in mcclGroupedGemm.  N a multiple of 8, K, ldx and ldw (bytes a row) of 16; values 16-byte, scales 4-byte aligned. */
+mcclResult_t mcclFp8Gemm(const void* x, int64_t ldx, const void* xScale, int64_t ldxScale, const void* w, int64_t ldw, const void* wScale,
+                         int64_t ldwScale, void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K, mcclStream_t stream);
+/* The same for bf16 x [rows, K] (16-byte aligned, ldx a multiple of 8), quantised into q [rows, K] (ldq bytes a row: a multiple of
+ * 16, best of 128, the width of a tile's rows) and its scales first. */
+mcclResult_t mcclFp8GemmBf16Rows(const void* x, int64_t ldx, void* q, int64_t ldq, void* qScale, int64_t ldqScale, const void* w, int64_t ldw,
+                                 const void* wScale, int64_t ldwScale, void* y, const void* ends, int ends64, int groups, int64_t rows, int N, int K,
                                  mcclStream_t stream);
 /* The smallest scale that brings a block's largest magnitude to 448 or less (a block of zeros: 1), and the nearest e4m3 numbers, of bf16
- * x [rows, K] by blocks of 128 of a row, and of contiguous x [outer, rows, K] by 128 x 128; q contiguous.  What is not finite becomes NaN. */
-mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, void* scale, int64_t ldScale, int64_t rows, int K, mcclStream_t stream);
-mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, void* scale, int64_t ldScale, int64_t outer, int rows, int K, mcclStream_t stream);
+ * x [rows, K] by blocks of 128 of a row, and of contiguous x [outer, rows, K] by 128 x 128; ldq bytes a row of q.  What is not finite becomes NaN. */
+mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, int64_t ldq, void* scale, int64_t ldScale, int64_t rows, int K,
+                                 mcclStream_t stream);
+mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, int64_t ldq, void* scale, int64_t ldScale, int64_t outer, int rows, int K, mcclStream_t stream);
 
 /* Fused all-gather -> GEMM -> activation.  xShard [M/n, K] in symmetric memory, xFull [M, K] local workspace,
  * W [N, K] local weight shard, out [M, N], flags >= 16 uint64 of device memory.  Collective over comm. */

@@ -19,8 +19,8 @@ BLOCK = 128
 
 class BlockScaled(NamedTuple):
     """`data` (float8_e4m3fn, [..., M, K]) and the scale of each block (float8_e8m0fnu, [..., M / rows, K / 128] rounded up), rows being
-    1 or 128.  `fp8_quantize` keeps the rows of the scales a multiple of four bytes apart, as the kernels read them; others are copied
-    into such rows in every call."""
+    1 or 128.  `fp8_quantize` keeps the rows of the scales a multiple of four bytes apart, as the kernels read them, and the rows of weights a
+    multiple of 128; scales of another pitch, and values whose rows are not a multiple of 16 bytes apart, are copied in every call."""
     data: torch.Tensor
     scale: torch.Tensor
 
@@ -36,7 +36,7 @@ def fp8_quantize(x: torch.Tensor, rows: int = 1) -> BlockScaled:
     """bf16 `x` in 8 bits: a scale for each 1 x 128 values of [M, K] (`rows=1`, activations) or for 128 x 128 of [N, K] or [E, N, K]
     (`rows=128`, weights).  The scale is the smallest power of two that brings the block's largest magnitude to 448 or less (1 for a block of
     zeros, never below 2^-127), the values the nearest e4m3 numbers of x / scale.  Inf and NaN take no part in the scale and become
-    NaN.  K is a multiple of 16; the last block of a row may be shorter than 128."""
+    NaN.  K is a multiple of 16; the last block of a row may be shorter than 128.  The result is a constant for autograd."""
     if rows not in (1, BLOCK):
         raise ValueError(f"fp8_quantize: blocks of 1 or {BLOCK} rows (got {rows})")
     if x.dtype != torch.bfloat16 or x.dim() not in ((2,) if rows == 1 else (2, 3)):

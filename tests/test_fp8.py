@@ -207,6 +207,12 @@ def test_strided_and_unaligned_operands():
         assert torch.equal(f.fp8_gemm(f.BlockScaled(data, xq.scale), wq), want)
     tight = lambda s: s.view(torch.uint8).contiguous().view(torch.float8_e8m0fnu)  # noqa: E731
     assert torch.equal(f.fp8_gemm(f.BlockScaled(xq.data, tight(xq.scale)), f.BlockScaled(wq.data, tight(wq.scale))), want)
+    # weights as they are quantised (rows a multiple of 128 apart), without gaps, and with rows no multiple of 16 apart
+    assert wq.data.stride(0) == 768
+    for pitch in (656, 661):
+        store = torch.empty(N, pitch, device="cuda", dtype=torch.uint8)
+        store[:, :K] = wq.data.view(torch.uint8)
+        assert torch.equal(f.fp8_gemm(xq, f.BlockScaled(store[:, :K].view(torch.float8_e4m3fn), wq.scale)), want)
     turned = f.BlockScaled(xq.data.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn),
                            xq.scale.view(torch.uint8).t().contiguous().t().view(torch.float8_e8m0fnu))
     assert torch.equal(f.fp8_gemm(turned, wq), want)
