@@ -30,6 +30,7 @@ constexpr int kScaleBase = 256;
 struct Args {
   CUtensorMap mapA;                    // x [M, K] bytes, box 128 x 128
   CUtensorMap mapB;                    // w [E, N, K] bytes, box 128 x BN
+  CUtensorMap mapC;                    // y [M, N], box 32 x 32
   const uint8_t *sx, *sw;              // [M][ldsx], [E][N / 128][ldsw]: scales, a row a multiple of four bytes apart
   int64_t ldsx, ldsw;
   const void* ends;                    // nullable: one group
@@ -120,6 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapA);
     umma::prefetchTensorMap(&a.mapB);
+    umma::prefetchTensorMap(&a.mapC);
   }
   if (warp == 2) { umma::tmemAlloc(tmemSlot, gemm::kTmemCols); umma::tmemRelinquish(); }
   if (warp == 3) grouped::readGroups(g, a.ends, a.ends64, a.groups, a.rows, BM, colTiles, lane);
@@ -247,9 +249,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
       if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);    // the sums are in registers: the next tile may start
       if (++acc == ACCS) { acc = 0; accPhase ^= 1; }
       const int r = tile.row + q * 32;
-      grouped::storeTile<COLS>(v, sStage + (warp - 4) * grouped::kStageBytes, a.out + ((size_t)g.start[tile.e] + r) * (size_t)a.N,
-                               g.start[tile.e + 1] - g.start[tile.e] - r, tile.col + half * COLS, a.N, lane);
+      grouped::storeTile<COLS>(v, sStage + (warp - 4) * grouped::kStageBytes, &a.mapC, tile.col + half * COLS, g.start[tile.e] + r, -1,
+                               a.out + ((size_t)g.start[tile.e] + r) * (size_t)a.N, g.start[tile.e + 1] - g.start[tile.e] - r, a.N, lane);
     }
+    if (lane == 0) umma::tmaStoreWaitAll();
     grouped::clearRows(a.out, g.start[a.groups], a.rows, a.N);
   }
 

@@ -37,6 +37,7 @@ enum Mode { FORWARD = 0, DATA = 1, WEIGHT = 2 };
 struct Args {
   CUtensorMap mapA;                    // FORWARD / DATA: x or dy [T, contracted], box 64 x 128; WEIGHT: dy [T, N], box 64 x 64
   CUtensorMap mapB;                    // FORWARD: w [E, N, K], box 64 x BN; DATA: the same, box 64 x 64; WEIGHT: x [T, K], box 64 x 64
+  CUtensorMap mapC;                    // the output: [T, width], box 32 x 32; WEIGHT: [E, N, K], box 32 x 32 x 1
   const void* ends;                    // [groups] int32 or int64
   int ends64, groups;
   int rows;                            // T
@@ -76,6 +77,12 @@ __device__ __forceinline__ void tmaLoad3d(void* smemDst, const CUtensorMap* map,
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       :: "r"(umma::smemAddr(smemDst)), "l"(map), "r"(umma::smemAddr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// Stores of a box from shared memory; elements outside the tensor are left out.
+__device__ __forceinline__ void tmaStore3d(const CUtensorMap* map, const void* smemSrc, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               :: "l"(map), "r"(umma::smemAddr(smemSrc)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
 // The groups as every role sees them: group e holds the rows [start[e], start[e + 1]); the tiles of all groups up to e number
@@ -136,14 +143,20 @@ __device__ __forceinline__ bool waitWarp(uint64_t* bar, uint32_t parity, uint64_
   return false;
 }
 
-// The epilogue of a warp: 32 rows (lane: row) x COLS sums as bf16, to `rows` rows from `out` on, `width` elements apart, columns from col0
-// on.  32 columns at a time go through 2 KB of shared memory, so that four lanes store 64 bytes of one row: a store from where the
-// sums are, a row per lane, touches 32 lines, and those take the SM longer than the products of a short contraction (64 experts of
-// 128 rows, dw of 2048 x 1024: 133 us; through shared memory 84 us).  16-byte pieces are swizzled over the rows: no bank is hit twice.
+// The epilogue of a warp: 32 rows (lane: row) x COLS sums as bf16, 32 columns at a time through 2 KB of shared memory, whose 16-byte pieces are
+// swizzled over the rows (as a tensor map's 64-byte swizzle does: no bank is hit twice).  Whole sets of 32 rows leave by TMA; a group's last
+// rows, up to `rows`, by stores of four lanes to 64 bytes of a row.  The epilogue runs beside the next tile's products and is what bounds short
+// contractions: 64 experts of 128 rows, dw of 2048 x 1024, a store from where the sums are, a row per lane, 133 us; all through shared memory and
+// lanes 72 us; by TMA 70 us.  16 experts of 512 rows, y of 512 x 2048: 36 and 35 us.
 template <int COLS>
-__device__ __forceinline__ void storeTile(const uint32_t* v, uint8_t* stage, __nv_bfloat16* out, int rows, int col0, int width, int lane) {
+__device__ __forceinline__ void storeTile(const uint32_t* v, uint8_t* stage, const CUtensorMap* map, int x, int y, int z, __nv_bfloat16* out, int rows, int width,
+                                          int lane) {
+  if (rows <= 0) return;
+  const bool byTma = z >= 0 || rows >= 32;
 #pragma unroll
   for (int c = 0; c < COLS / 32; ++c) {
+    if (x + 32 * c >= width) break;
+    if (lane == 0) umma::tmaStoreWaitRead<0>();            // what left this memory before has been read
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -154,13 +167,22 @@ __device__ __forceinline__ void storeTile(const uint32_t* v, uint8_t* stage, __n
         o2[i] = __floats2bfloat162_rn(__uint_as_float(v[32 * c + 8 * j + 2 * i]), __uint_as_float(v[32 * c + 8 * j + 2 * i + 1]));
       *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = o;
     }
-    __syncwarp();
-    const int col = col0 + 32 * c + (lane & 3) * 8;
+    if (byTma) {
+      umma::fenceProxyAsyncShared();
+      __syncwarp();
+      if (lane == 0) {
+        if (z >= 0) tmaStore3d(map, stage, x + 32 * c, y, z); else umma::tmaStore2d(map, stage, x + 32 * c, y);
+        umma::tmaStoreCommit();
+      }
+    } else {
+      __syncwarp();
+      const int col = x + 32 * c + (lane & 3) * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      const uint4 o = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-      if (r < rows && col < width) *reinterpret_cast<uint4*>(out + (size_t)r * width + col) = o;
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        const uint4 o = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+        if (r < rows && col < width) *reinterpret_cast<uint4*>(out + (size_t)r * width + col) = o;
+      }
     }
   }
 }
@@ -213,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapA);
     umma::prefetchTensorMap(&a.mapB);
+    umma::prefetchTensorMap(&a.mapC);
   }
   if (warp == 2) { umma::tmemAlloc(tmemSlot, gemm::kTmemCols); umma::tmemRelinquish(); }
   if (warp == 3) readGroups(g, a.ends, a.ends64, a.groups, a.rows, MODE == WEIGHT ? 0 : BM, MODE == WEIGHT ? wRowTiles * colTiles : colTiles, lane);
@@ -341,8 +364,10 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       __syncwarp();
       if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
       acc ^= 1; if (acc == 0) accPhase ^= 1;
-      storeTile<COLS>(v, sStage + (warp - 4) * kStageBytes, out, limit - r, tile.col + half * COLS, a.width, lane);
+      storeTile<COLS>(v, sStage + (warp - 4) * kStageBytes, &a.mapC, tile.col + half * COLS, MODE == WEIGHT ? r : g.start[tile.e] + r,
+                      MODE == WEIGHT ? tile.e : -1, out, limit - r, a.width, lane);
     }
+    if (lane == 0) umma::tmaStoreWaitAll();
     if (MODE != WEIGHT) clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }
 

@@ -23,22 +23,33 @@ int mccl::gemm::pickColumns(double rowTiles, int width, int sms) {
   return waves(128) * 0.8 < waves(256) ? 128 : 256;
 }
 
-mcclResult_t mccl::gemm::rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld,
-                                 uint32_t boxRows) {
-  static EncodeTiledFn fn = encodeTiled();
+namespace {
+
+mcclResult_t encode(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxCols,
+                    uint32_t boxRows, CUtensorMapSwizzle swizzle) {
+  static gemm::EncodeTiledFn fn = gemm::encodeTiled();
   if (fn == nullptr) MCCLFAIL(mcclSystemError);
   const cuuint64_t dims[3] = {cols, rows, outer};
   const cuuint64_t strides[2] = {ld * elementBytes, rows * ld * elementBytes};
-  const cuuint32_t box[3] = {(cuuint32_t)(128 / elementBytes), boxRows, 1}, elemStrides[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {boxCols, boxRows, 1}, elemStrides[3] = {1, 1, 1};
   const CUresult r = fn(map, elementBytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, outer ? 3 : 2, const_cast<void*>(base), dims,
-                        strides, box, elemStrides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        strides, box, elemStrides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     MCCL_WARN("cuTensorMapEncodeTiled failed with %d (base %p, %llu x %llu x %llu, row pitch %llu)", (int)r, base, (unsigned long long)outer,
               (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)ld);
     return mcclInvalidArgument;
   }
   return mcclSuccess;
+}
+
+}  // namespace
+
+mcclResult_t mccl::gemm::rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld,
+                                 uint32_t boxRows) {
+  return encode(map, base, elementBytes, outer, rows, cols, ld, 128 / elementBytes, boxRows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+mcclResult_t mccl::gemm::outputMap(CUtensorMap* map, void* base, uint64_t outer, uint64_t rows, uint64_t cols) {
+  return encode(map, base, 2, outer, rows, cols, cols, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 namespace {
@@ -119,6 +130,7 @@ mcclResult_t weightGradient(const void* dy, int64_t lddy, const void* x, int64_t
   MCCLCHECK(gemm::rowsMap(&a.mapB, x, 2, 0, rows, K, ldx, 64));
   a.tileRows = N; a.width = K;
   a.out = static_cast<__nv_bfloat16*>(dw);
+  MCCLCHECK(gemm::outputMap(&a.mapC, dw, groups, N, K));
   return run<WEIGHT>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn, beside);
 }
 
@@ -150,6 +162,7 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, bn));
   a.contracted = K; a.width = N;
   a.out = static_cast<__nv_bfloat16*>(y);
+  MCCLCHECK(gemm::outputMap(&a.mapC, y, 0, rows, N));
   return run<FORWARD>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
 }
 
@@ -170,6 +183,7 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, 64));
   a.contracted = N; a.width = K;
   a.out = static_cast<__nv_bfloat16*>(dx);
+  MCCLCHECK(gemm::outputMap(&a.mapC, dx, 0, rows, K));
   return run<DATA>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
 }
 

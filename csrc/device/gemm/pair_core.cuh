@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapA);
     umma::prefetchTensorMap(&a.mapB);
+    umma::prefetchTensorMap(&a.mapC);
   }
   if (warp == 2) { gemm::umma2::tmemAlloc(tmemSlot, gemm::kTmemCols); gemm::umma2::tmemRelinquish(); }
   if (warp == 3) grouped::readGroups(g, a.ends, a.ends64, a.groups, a.rows, MODE == WEIGHT ? 0 : kRows, MODE == WEIGHT ? wRowTiles * colTiles : colTiles, lane);
@@ -238,8 +239,10 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
       __syncwarp();
       if (lane == 0) thin::arriveCluster(&tmemEmpty[acc], 0);
       acc ^= 1; if (acc == 0) accPhase ^= 1;
-      grouped::storeTile<HALF>(v, stage, out, limit - r, tile.col + half * HALF, a.width, lane);
+      grouped::storeTile<HALF>(v, stage, &a.mapC, tile.col + half * HALF, MODE == WEIGHT ? r : g.start[tile.e] + r, MODE == WEIGHT ? tile.e : -1, out, limit - r,
+                               a.width, lane);
     }
+    if (lane == 0) umma::tmaStoreWaitAll();
     if (MODE != WEIGHT) grouped::clearRows(a.out, g.start[a.groups], a.rows, a.width);
   }
 
