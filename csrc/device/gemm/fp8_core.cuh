@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
   const uint32_t tmemBase = *tmemSlot;
   const int totalTiles = g.prefix[a.groups];
   auto at = [&](int t, int* e, Tile* tile) {               // tile t; `e` is carried from the tile before
-    while (t >= g.prefix[*e + 1]) ++*e;
+    *e = grouped::groupOf(g, t, *e, a.groups);
     grouped::tileAt(g, t, *e, (g.start[*e + 1] - g.start[*e] + BM - 1) / BM, colTiles, BM, BN, tile);
   };
 

@@ -100,27 +100,47 @@ __device__ __forceinline__ void readGroups(const Groups& g, const void* ends, in
     if (lane == 0) { g.start[1] = T; g.prefix[1] = (T + rowTile - 1) / rowTile * perRowTile; }
     return;
   }
-  for (int e0 = 0; e0 < groups; e0 += 32) {
-    const int e = e0 + lane;
-    int end = 0;
-    if (e < groups) {
-      const int64_t v = ends64 ? static_cast<const int64_t*>(ends)[e] : (int64_t) static_cast<const int32_t*>(ends)[e];
-      end = (int)(v < 0 ? 0 : v > T ? T : v);
+  // Eight rounds' ends are asked for at a time (1024 groups: one round after another 40 us a product, so 35 us, by halves below 15 us).
+  constexpr int ROUNDS = 8;
+  for (int base = 0; base < groups; base += 32 * ROUNDS) {
+    int v[ROUNDS];
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+      const int e = base + 32 * u + lane;
+      int64_t w = 0;
+      if (e < groups) w = ends64 ? static_cast<const int64_t*>(ends)[e] : (int64_t) static_cast<const int32_t*>(ends)[e];
+      v[u] = (int)(w < 0 ? 0 : w > T ? T : w);
     }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, end, o); if (lane >= o && v > end) end = v; }
-    if (end < last) end = last;
-    int begin = __shfl_up_sync(0xffffffffu, end, 1);
-    if (lane == 0) begin = last;
-    int n = e < groups ? (rowTile == 0 ? perRowTile : (end - begin + rowTile - 1) / rowTile * perRowTile) : 0;
+    for (int u = 0; u < ROUNDS; ++u) {
+      if (base + 32 * u >= groups) break;
+      const int e = base + 32 * u + lane;
+      int end = v[u];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += v; }
-    if (e < groups) { g.start[e + 1] = end; g.prefix[e + 1] = tiles + n; }
-    last = __shfl_sync(0xffffffffu, end, 31);
-    tiles += __shfl_sync(0xffffffffu, n, 31);
+      for (int o = 1; o < 32; o <<= 1) { const int w = __shfl_up_sync(0xffffffffu, end, o); if (lane >= o && w > end) end = w; }
+      if (end < last) end = last;
+      int begin = __shfl_up_sync(0xffffffffu, end, 1);
+      if (lane == 0) begin = last;
+      int n = e < groups ? (rowTile == 0 ? perRowTile : (end - begin + rowTile - 1) / rowTile * perRowTile) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int w = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += w; }
+      if (e < groups) { g.start[e + 1] = end; g.prefix[e + 1] = tiles + n; }
+      last = __shfl_sync(0xffffffffu, end, 31);
+      tiles += __shfl_sync(0xffffffffu, n, 31);
+    }
   }
 }
 
+// The group of tile t, from that of an earlier tile on; by halves, as many groups may have no rows (1024 of them one by one: 20 us).
+__device__ __forceinline__ int groupOf(const Groups& g, int t, int e, int groups) {
+  if (t < g.prefix[e + 1]) return e;
+  int lo = e + 1, hi = groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (t < g.prefix[mid + 1]) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
 // Tile t of all, which is one of group e: its first row and first column.  The tiles of a group go panel by panel of eight row tiles, the row
 // fastest, so that what runs at a time shares a few weight tiles.
 struct Tile { int e, row, col; };
@@ -252,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       tileAt(g, t, *e, wRowTiles, colTiles, BM, BN, tile);
       return (g.start[*e + 1] - g.start[*e] + CK - 1) / CK;
     } else {
-      while (t >= g.prefix[*e + 1]) ++*e;
+      *e = groupOf(g, t, *e, a.groups);
       tileAt(g, t, *e, (g.start[*e + 1] - g.start[*e] + BM - 1) / BM, colTiles, BM, BN, tile);
       return kBlocks;
     }
@@ -304,9 +324,12 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       umma::tcFenceAfter();
       const uint32_t d = tmemBase + (uint32_t)acc * 256u;
       bool ok = true;
-      for (int kb = 0; kb < blocks; ++kb) {
+      for (int kb = 0; kb < blocks && ok; ++kb) {
         ok = umma::mbarWait(&full[stage], phase, budget);
-        if (!ok) break;
+        if (MODE == WEIGHT) {                              // the lanes meet below: they leave together
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
         uint8_t *pa = sA + stage * S::A_BYTES, *pb = sB + stage * S::B_BYTES;
         const bool behind = MODE == WEIGHT && tail != 0 && kb == blocks - 1;
         if (behind) {
@@ -320,8 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
             for (int c = 0; c < BN / 64; ++c) *reinterpret_cast<uint4*>(pb + c * 8192 + off) = make_uint4(0, 0, 0, 0);
           }
           umma::fenceProxyAsyncShared();
+          __syncwarp();
         }
-        __syncwarp();
         umma::tcFenceAfter();
         if (issues) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));

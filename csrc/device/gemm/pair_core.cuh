@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
       grouped::tileAt(g, t, *e, wRowTiles, colTiles, kRows, BN, tile);
       return (g.start[*e + 1] - g.start[*e] + CK - 1) / CK;
     } else {
-      while (t >= g.prefix[*e + 1]) ++*e;
+      *e = grouped::groupOf(g, t, *e, a.groups);
       grouped::tileAt(g, t, *e, (g.start[*e + 1] - g.start[*e] + kRows - 1) / kRows, colTiles, kRows, BN, tile);
       return kBlocks;
     }

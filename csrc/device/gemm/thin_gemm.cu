@@ -60,10 +60,11 @@ int64_t expertsWithRows(int64_t rows, int groups) { return std::min<int64_t>(row
 // Where a tile's contraction can be shared by two CTAs or more (8 bits, 100 rows of 8192 by 11008 columns, which cannot: 32 us here, 21 us in tiles of
 // 128 rows), and for up to 32 rows whose weights' rows are not short (one row of 4096 by 22016 columns 14.5 us here, 26 us there; of 1024 by
 // 50304 columns 14.4 and 12.9 us).  With groups, whose rows the host does not know: where the tiles of 128 rows x 128 columns are no more than
-// the SMs (64 rows for 32 experts of 2048 x 5504, which are more: 106 us here, 103 us there).
+// the SMs (64 rows for 32 experts of 2048 x 5504, which are more: 106 us here, 103 us there), and the CTAs that find no rows are few (two rows, 64
+// experts of 2048 x 1024 in 8 bits: 10.6 us here, 9.0 us there).
 bool mccl::gemm::thinWanted(int64_t rows, bool ragged, int groups, int N, int64_t kBytes) {
   const int64_t nTiles = (N + BM - 1) / BM, sms = gemmSmCount();
-  if (ragged) return (rows / BM + expertsWithRows(rows, groups)) * nTiles <= sms;
+  if (ragged) return (rows / BM + expertsWithRows(rows, groups)) * nTiles <= sms && groups * nTiles <= 2 * sms;
   if (rows <= 32) return nTiles <= sms || kBytes >= 2048;
   return 2 * nTiles * ((rows + 63) / 64) <= placesFor(sms);
 }
