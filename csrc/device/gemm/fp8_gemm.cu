@@ -62,7 +62,7 @@ mcclResult_t product(const void* x, int64_t ldx, const void* xScale, int64_t ldx
   memset(&a, 0, sizeof(a));
   MCCLCHECK(gemm::rowsMap(&a.mapA, x, 1, 0, rows, K, ldx, BM));
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 1, groups, N, K, ldw, bn));
-  MCCLCHECK(gemm::outputMap(&a.mapC, y, 0, rows, N));
+  MCCLCHECK(gemm::outputMap(&a.mapC, y, 0, rows, N, 32));
   a.sx = static_cast<const uint8_t*>(xScale);
   a.sw = static_cast<const uint8_t*>(wScale);
   a.ldsx = ldxScale; a.ldsw = ldwScale;

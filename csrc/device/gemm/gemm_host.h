@@ -58,8 +58,8 @@ int pickColumns(double rowTiles, int width, int sms);
 // Tensor map of [outer][rows][cols] (outer 0: a matrix) of 2-byte (bf16) or 1-byte elements, rows `ld` elements apart: boxes of 128 bytes x
 // boxRows, 128-byte swizzle, zeros outside.
 mcclResult_t rowsMap(CUtensorMap* map, const void* base, int elementBytes, uint64_t outer, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t boxRows);
-// Of the output, contiguous bf16 [outer][rows][cols] (outer 0: a matrix): boxes of 32 columns x 32 rows, 64-byte swizzle.
-mcclResult_t outputMap(CUtensorMap* map, void* base, uint64_t outer, uint64_t rows, uint64_t cols);
+// Of the output, contiguous bf16 [outer][rows][cols] (outer 0: a matrix): boxes of 32 or 64 columns x 32 rows, swizzled over their width.
+mcclResult_t outputMap(CUtensorMap* map, void* base, uint64_t outer, uint64_t rows, uint64_t cols, int boxCols);
 
 }  // namespace gemm
 }  // namespace mccl

@@ -37,7 +37,7 @@ enum Mode { FORWARD = 0, DATA = 1, WEIGHT = 2 };
 struct Args {
   CUtensorMap mapA;                    // FORWARD / DATA: x or dy [T, contracted], box 64 x 128; WEIGHT: dy [T, N], box 64 x 64
   CUtensorMap mapB;                    // FORWARD: w [E, N, K], box 64 x BN; DATA: the same, box 64 x 64; WEIGHT: x [T, K], box 64 x 64
-  CUtensorMap mapC;                    // the output: [T, width], box 32 x 32; WEIGHT: [E, N, K], box 32 x 32 x 1
+  CUtensorMap mapC;                    // the output: [T, width], box 32 x 32; WEIGHT: [E, N, K], box 32 x 32 x 1, WHOLE 64 x 32 x 1
   const void* ends;                    // [groups] int32 or int64
   int ends64, groups;
   int rows;                            // T
@@ -48,12 +48,14 @@ struct Args {
   uint64_t budgetNs;
 };
 
-template <int BN> struct Smem {
+template <int BN, bool WHOLE> struct Smem {
   static constexpr int A_BYTES = BM * kStageK, B_BYTES = BN * kStageK;
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  // WHOLE: a stage less, for an epilogue that has a warp's whole part of a tile in shared memory (storeWhole).
+  static constexpr int STAGES = BN == 256 ? (WHOLE ? 3 : 4) : (WHOLE ? 5 : 6);
   static constexpr int TILE_BYTES = STAGES * (A_BYTES + B_BYTES);
+  static constexpr int EPI_BYTES = WHOLE ? 32 * BN : kStageBytes;                    // a warp: 32 rows x BN / 2 columns of bf16
   static constexpr int TABLE_BYTES = 2 * (kMaxGroups + 4) * 4;
-  static constexpr int TOTAL = TILE_BYTES + kEpiWarps * kStageBytes + TABLE_BYTES + 256 + 1024;
+  static constexpr int TOTAL = TILE_BYTES + kEpiWarps * EPI_BYTES + TABLE_BYTES + 256 + 1024;
 };
 
 // The two products of a backward pass read the same dy and need nothing of each other: the second is launched with programmatic stream
@@ -206,6 +208,32 @@ __device__ __forceinline__ void storeTile(const uint32_t* v, uint8_t* stage, con
     }
   }
 }
+// The same for the gradient of the weights of experts with few rows, whose contraction is one block: all COLS columns in shared memory at a time, one
+// wait, one fence and a box of 64 columns or two in place of four of each, for one stage less.  32 experts of 2048 x 5504 with two rows each
+// 143 -> 126 us, 64 of 520 x 776 with 47 rows 31 -> 28 us; but with 128 rows each (1024 x 2048) 69 -> 75 us, 16 with 512 rows 39 -> 45 us.
+template <int COLS>
+__device__ __forceinline__ void storeWhole(const uint32_t* v, uint8_t* stage, const CUtensorMap* map, int x, int y, int z, int rows, int width, int lane) {
+  if (rows <= 0 || x >= width) return;
+  if (lane == 0) umma::tmaStoreWaitRead<0>();
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < COLS / 8; ++j) {
+    uint4 o;
+    __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o2[i] = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+    *reinterpret_cast<uint4*>(stage + j / 8 * 4096 + lane * 128 + (((j & 7) ^ (lane & 7)) << 4)) = o;
+  }
+  umma::fenceProxyAsyncShared();
+  __syncwarp();
+  if (lane == 0) {
+#pragma unroll
+    for (int b = 0; b < COLS / 64; ++b)
+      if (x + 64 * b < width) tmaStore3d(map, stage + b * 4096, x + 64 * b, y, z);
+    umma::tmaStoreCommit();
+  }
+}
+
 // Zeros in a warp's 32 rows x COLS columns.
 template <int COLS>
 __device__ __forceinline__ void clearTile(__nv_bfloat16* out, int rows, int col0, int width, int lane) {
@@ -222,9 +250,10 @@ __device__ __forceinline__ void clearRows(__nv_bfloat16* out, int from, int to, 
     reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
 }
 
-template <int BN, int MODE>
+template <int BN, int MODE, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_constant__ Args a) {
-  using S = Smem<BN>;
+  static_assert(!WHOLE || MODE == WEIGHT, "storeWhole leaves the rows behind an expert's last out by the tensor map");
+  using S = Smem<BN, WHOLE>;
   constexpr int ST = S::STAGES;
   constexpr int CK = 64;                                   // contracted elements a stage
   extern __shared__ uint8_t smemRaw[];
@@ -232,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
   uint8_t* sA = smem;
   uint8_t* sB = smem + ST * S::A_BYTES;
   uint8_t* sStage = smem + S::TILE_BYTES;
-  int* table = reinterpret_cast<int*>(sStage + kEpiWarps * kStageBytes);
+  int* table = reinterpret_cast<int*>(sStage + kEpiWarps * S::EPI_BYTES);
   const Groups g{table, table + kMaxGroups + 4};
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + S::TABLE_BYTES);
   uint64_t* full = bars;                                   // [ST] TMA -> MMA
@@ -387,8 +416,10 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
       __syncwarp();
       if (lane == 0) umma::mbarArrive(&tmemEmpty[acc]);
       acc ^= 1; if (acc == 0) accPhase ^= 1;
-      storeTile<COLS>(v, sStage + (warp - 4) * kStageBytes, &a.mapC, tile.col + half * COLS, MODE == WEIGHT ? r : g.start[tile.e] + r,
-                      MODE == WEIGHT ? tile.e : -1, out, limit - r, a.width, lane);
+      uint8_t* stage = sStage + (warp - 4) * S::EPI_BYTES;
+      if (WHOLE) storeWhole<COLS>(v, stage, &a.mapC, tile.col + half * COLS, r, tile.e, limit - r, a.width, lane);
+      else storeTile<COLS>(v, stage, &a.mapC, tile.col + half * COLS, MODE == WEIGHT ? r : g.start[tile.e] + r, MODE == WEIGHT ? tile.e : -1, out, limit - r,
+                           a.width, lane);
     }
     if (lane == 0) umma::tmaStoreWaitAll();
     if (MODE != WEIGHT) clearRows(a.out, g.start[a.groups], a.rows, a.width);

@@ -48,8 +48,8 @@ mcclResult_t mccl::gemm::rowsMap(CUtensorMap* map, const void* base, int element
                                  uint32_t boxRows) {
   return encode(map, base, elementBytes, outer, rows, cols, ld, 128 / elementBytes, boxRows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-mcclResult_t mccl::gemm::outputMap(CUtensorMap* map, void* base, uint64_t outer, uint64_t rows, uint64_t cols) {
-  return encode(map, base, 2, outer, rows, cols, cols, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+mcclResult_t mccl::gemm::outputMap(CUtensorMap* map, void* base, uint64_t outer, uint64_t rows, uint64_t cols, int boxCols) {
+  return encode(map, base, 2, outer, rows, cols, cols, boxCols, 32, boxCols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 namespace {
@@ -63,18 +63,18 @@ int boundDevice() {
   return dev;
 }
 
-template <int BN, int MODE>
+template <int BN, int MODE, bool WHOLE>
 mcclResult_t launchAs(const Args& a, int dev, int grid, bool beside, cudaStream_t s) {
-  auto* kernel = groupedKernel<BN, MODE>;
+  auto* kernel = groupedKernel<BN, MODE, WHOLE>;
   static std::atomic<uint64_t> prepared{0};                // a bit per device: the attribute stays with the function
   if (!(prepared.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BN>::TOTAL) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (Smem<BN, WHOLE>::TOTAL)) != cudaSuccess) { cudaGetLastError(); return mcclSystemError; }
     prepared.fetch_or(1ull << (dev & 63));
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Smem<BN>::TOTAL;
+  cfg.dynamicSmemBytes = (Smem<BN, WHOLE>::TOTAL);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -94,7 +94,7 @@ bool valid(const Shape& s) {
 }
 bool validRows(const void* p, int64_t ld, int cols) { return p != nullptr && aligned16(p) && ld >= cols && ld % 8 == 0; }
 
-template <int MODE>
+template <int MODE, bool WHOLE = false>
 mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn, bool beside = false) {
   a.errFlag = gemm::gemmErrFlag(dev);
   if (a.errFlag == nullptr) return mcclSystemError;
@@ -103,7 +103,7 @@ mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_
   const int64_t tiles = rowTiles * ((a.width + bn - 1) / bn);
   if (tiles > INT32_MAX) return mcclInvalidArgument;
   const int sms = gemm::gemmSmCount(), grid = (int)(tiles < sms ? tiles : sms);
-  return bn == 256 ? launchAs<256, MODE>(a, dev, grid, beside, stream) : launchAs<128, MODE>(a, dev, grid, beside, stream);
+  return bn == 256 ? launchAs<256, MODE, WHOLE>(a, dev, grid, beside, stream) : launchAs<128, MODE, WHOLE>(a, dev, grid, beside, stream);
 }
 
 // Row tiles of all groups: at most one beside the full ones for each group.
@@ -130,8 +130,10 @@ mcclResult_t weightGradient(const void* dy, int64_t lddy, const void* x, int64_t
   MCCLCHECK(gemm::rowsMap(&a.mapB, x, 2, 0, rows, K, ldx, 64));
   a.tileRows = N; a.width = K;
   a.out = static_cast<__nv_bfloat16*>(dw);
-  MCCLCHECK(gemm::outputMap(&a.mapC, dw, groups, N, K));
-  return run<WEIGHT>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn, beside);
+  const bool whole = rows <= 64 * (int64_t)groups;         // one block of rows an expert on the average
+  MCCLCHECK(gemm::outputMap(&a.mapC, dw, groups, N, K, whole ? 64 : 32));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return whole ? run<WEIGHT, true>(a, s, dev, rt, st, bn, beside) : run<WEIGHT>(a, s, dev, rt, st, bn, beside);
 }
 
 }  // namespace
@@ -162,7 +164,7 @@ mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y,
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, bn));
   a.contracted = K; a.width = N;
   a.out = static_cast<__nv_bfloat16*>(y);
-  MCCLCHECK(gemm::outputMap(&a.mapC, y, 0, rows, N));
+  MCCLCHECK(gemm::outputMap(&a.mapC, y, 0, rows, N, 32));
   return run<FORWARD>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
 }
 
@@ -183,7 +185,7 @@ mcclResult_t mcclGroupedGemmBackwardData(const void* dy, int64_t lddy, const voi
   MCCLCHECK(gemm::rowsMap(&a.mapB, w, 2, groups, N, K, K, 64));
   a.contracted = N; a.width = K;
   a.out = static_cast<__nv_bfloat16*>(dx);
-  MCCLCHECK(gemm::outputMap(&a.mapC, dx, 0, rows, K));
+  MCCLCHECK(gemm::outputMap(&a.mapC, dx, 0, rows, K, 32));
   return run<DATA>(a, s, dev, rt, reinterpret_cast<cudaStream_t>(stream), bn);
 }
 

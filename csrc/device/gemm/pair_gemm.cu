@@ -64,7 +64,7 @@ mcclResult_t mccl::gemm::pairGemm(const PairCall& c, int device, void* stream) {
     MCCLCHECK(rowsMap(&a.mapA, c.a, 2, 0, c.rows, c.mode == DATA ? c.N : c.K, c.lda, BM));
     MCCLCHECK(rowsMap(&a.mapB, c.b, 2, c.groups, c.N, c.K, c.K, c.mode == DATA ? 64 : HALF));
   }
-  MCCLCHECK(outputMap(&a.mapC, c.out, c.mode == WEIGHT ? c.groups : 0, c.mode == WEIGHT ? c.N : c.rows, width));
+  MCCLCHECK(outputMap(&a.mapC, c.out, c.mode == WEIGHT ? c.groups : 0, c.mode == WEIGHT ? c.N : c.rows, width, 32));
   a.ends = c.ends; a.ends64 = c.ends64; a.groups = c.groups;
   a.rows = (int)c.rows;
   a.contracted = c.mode == DATA ? c.N : c.K;
