@@ -52,7 +52,11 @@ constexpr int kPieces = 4, kPerBlock = 8;
 template <class I>
 __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat16* x, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int64_t rows,
                                                                int K, int blocks) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // a product behind this may start; it waits for this grid's end where it reads
+  // Launched with programmatic stream serialization, which hides its launch behind the end of what runs before; everything here comes after
+  // that.  Then a product behind this may start, which itself waits for this grid's end where it reads what it makes.  (One row of 4096 by
+  // 11008 columns, quantised and multiplied, call after call: 14.9 -> 13.3 us.)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const I total = (I)rows * (I)blocks, b0 = (I)blockIdx.x * (kThreads / kPerBlock * kPieces) + (threadIdx.x / kPerBlock);
   const int in = (threadIdx.x % kPerBlock) * 16;
   uint4 v[kPieces][2];
@@ -129,8 +133,16 @@ mcclResult_t mcclFp8QuantizeRows(const void* x, int64_t ldx, void* q, int64_t ld
   if (!x || !q || !scale || !aligned16(x) || !aligned16(q) || rows * blocks > (int64_t)INT32_MAX * 16) return mcclInvalidArgument;
   const int64_t per = kThreads / kPerBlock * kPieces, ctas = (rows * blocks + per - 1) / per;
   auto* kernel = rows * blocks < (1ll << 31) - per ? quantizeRowsKernel<uint32_t> : quantizeRowsKernel<int64_t>;
-  kernel<<<(unsigned)ctas, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q),
-                                                                                  ldq, static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<const __nv_bfloat16*>(x), ldx, static_cast<uint8_t*>(q), ldq, static_cast<uint8_t*>(scale), ldScale, rows, K, blocks);
   return launchedOk();
 }
 

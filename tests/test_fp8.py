@@ -279,3 +279,45 @@ def test_refusals():
     for args in ((x, 2), (x.float(),), (x[0],), (x[None],), (x[:, :40],), (x[:, :0],), (x[None, None], 128), (x[:0], 128)):
         with pytest.raises(ValueError):
             f.fp8_quantize(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 40, 2500])
+def test_calls_right_behind_what_makes_their_operands(M):
+    """Kernels of a call start before those in front of them have ended: rows, weights and ends that are written just before, by a long
+    kernel, and results that are read just behind, over memory that is used again and again."""
+    f = _fp8()
+    N, K = 264, 528
+    rows, weights = [_scaled(M, K) for _ in range(4)], [f.fp8_quantize(_bf(2, N, K), 128) for _ in range(4)]
+    ends = [torch.tensor([i, M], device="cuda") for i in range(4)]
+    want = [[f.fp8_gemm(x, w, e).clone() for x, e in zip(rows, ends)] for w in weights]
+    torch.cuda.synchronize()
+    x, e = torch.empty_like(rows[0]), torch.empty_like(ends[0])
+    w = f.BlockScaled(torch.empty_like(weights[0].data), torch.empty_like(weights[0].scale))
+    big = torch.randn(4096, 4096, device="cuda")
+    wrong = torch.zeros((), device="cuda")
+    for turn in range(40):
+        i, j = turn % 4, turn // 4 % 4
+        big = big @ big * 1e-2                                       # what follows is queued while this runs
+        x.copy_(rows[i])
+        e.copy_(ends[i])
+        w.data.view(torch.uint8).copy_(weights[j].data.view(torch.uint8))
+        w.scale.view(torch.uint8).copy_(weights[j].scale.view(torch.uint8))
+        y = f.fp8_gemm(x, w, e)
+        wrong += (y != want[j][i]).sum()
+        del y
+    assert wrong.item() == 0
+
+
+@pytest.mark.gpu
+def test_large_product_from_a_graph():
+    f = _fp8()
+    x, w = _scaled(2500, 528), f.fp8_quantize(_bf(1032, 528), 128)
+    want = f.fp8_gemm(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f.fp8_gemm(x, w)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)

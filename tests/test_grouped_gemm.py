@@ -213,6 +213,32 @@ def test_same_bits_on_another_stream_and_from_a_graph():
     assert last_error() == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,K,N", [([9, 0, 30], 264, 200), ([700, 0, 1900], 520, 1032), ([2500, 2700], 1032, 2312)])
+def test_gradients_right_behind_what_makes_them(sizes, K, N):
+    """The second product of a backward pass runs beside the first one: operands written just before, results read just behind, over memory that
+    is used again and again."""
+    T, E = sum(sizes), len(sizes)
+    xs, ws, dys = [_bf(T, K) for _ in range(3)], [_bf(E, N, K) for _ in range(3)], [_bf(T, N) for _ in range(3)]
+    ends = torch.tensor(sizes, device="cuda").cumsum(0)
+    want = [_run(x, w, ends, dy) for x, w, dy in zip(xs, ws, dys)]
+    torch.cuda.synchronize()
+    x, w, dy = torch.empty_like(xs[0]).requires_grad_(True), torch.empty_like(ws[0]).requires_grad_(True), torch.empty_like(dys[0])
+    big, wrong = torch.randn(4096, 4096, device="cuda"), torch.zeros((), device="cuda")
+    for turn in range(30):
+        i = turn % 3
+        big = big @ big * 1e-2                                       # what follows is queued while this runs
+        with torch.no_grad():
+            x.copy_(xs[i])
+            w.copy_(ws[i])
+            dy.copy_(dys[i])
+        y = _gg(x, w, ends)
+        dx, dw = torch.autograd.grad(y, [x, w], dy)
+        wrong += (y != want[i][0]).sum() + (dx != want[i][1]).sum() + (dw != want[i][2]).sum()
+        del y, dx, dw
+    assert wrong.item() == 0
+
+
 def test_refusals():
     x, w, ends = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(2, 8, 16, dtype=torch.bfloat16), torch.tensor([2, 4])
     with pytest.raises(RuntimeError, match="CUDA"):
