@@ -96,7 +96,7 @@ py::object fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const T
   } else {
     // One buffer for the quantised rows and, behind them, their scales.  Rows begin at whole lines: a tile's rows of 128 bytes that lie
     // across two lines take about twice as long to load (5003 rows of 2064 through 16 experts of 5504: 104 -> 93 us;
-    // with the weights laid out so, too, 86 us).
+    // with the weights laid out so, too, 82 us).
     const int64_t pitch = blocksOf(K) * kBlock, ld = (blocksOf(K) + 3) / 4 * 4;
     Tensor work = at::empty({M * (pitch + ld)}, x.options().dtype(at::kByte));
     char* q = static_cast<char*>(work.data_ptr());
