@@ -271,7 +271,8 @@ class DroplessMoE(nn.Module):
 
 class QuantizedMoE(DroplessMoE):
     """DroplessMoE with its experts in 8 bits with a scale for each block of 128 (ops/fp8.py), for serving: no gradients.  Made by
-    `DroplessMoE.quantized()`; hidden and ffn are multiples of 16, tokens bf16 on CUDA."""
+    `DroplessMoE.quantized()`; hidden and ffn are multiples of 16, tokens bf16 on CUDA.  The 8-bit experts are neither parameters nor buffers:
+    they stay on their GPU and in no state_dict, which holds the router alone; keep the DroplessMoE's and quantise again."""
 
     def __init__(self, layer: DroplessMoE):
         from ..ops.fp8 import fp8_quantize

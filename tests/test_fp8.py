@@ -321,3 +321,46 @@ def test_large_product_from_a_graph():
         out.zero_()
         graph.replay()
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before", ["nothing", "copy", "from_host", "memset", "join", "join_of_a_copy"])
+def test_captured_behind_other_work(before):
+    """The kernel that quantises starts early behind what is in front of it, whatever that is in a graph: nothing, a kernel, a copy from the
+    host, a memset, another stream's work."""
+    f = _fp8()
+    source, w = _scaled(48, 528), f.fp8_quantize(_bf(264, 528), 128)
+    host, x, big = source.cpu().pin_memory(), torch.empty_like(source), torch.randn(1 << 24, device="cuda")
+    want = f.fp8_gemm(torch.zeros_like(source) if before == "memset" else source, w)
+
+    def call():
+        if before == "nothing":
+            return f.fp8_gemm(source, w)
+        if before == "copy":
+            x.copy_(source)
+        elif before == "from_host":
+            x.copy_(host, non_blocking=True)
+        elif before == "memset":
+            x.zero_()
+        else:
+            here, side = torch.cuda.current_stream(), torch.cuda.Stream()
+            side.wait_stream(here)
+            with torch.cuda.stream(side):
+                big.mul_(1.0)                                        # long beside what follows here
+                x.copy_(host if before == "join_of_a_copy" else source, non_blocking=True)
+            if before == "join":
+                big.sum()
+            here.wait_stream(side)
+        return f.fp8_gemm(x, w)
+
+    x.fill_(7)
+    assert torch.equal(call(), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(3):
+        x.fill_(7)
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
