@@ -364,3 +364,19 @@ def test_captured_behind_other_work(before):
         out.zero_()
         graph.replay()
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,E,N,K", [(280000, 1, 136, 8192), (280000, 1, 8192, 272), (900, 33, 8192, 8192)])
+def test_more_elements_than_32_bits_count(M, E, N, K):
+    """Rows, results and weights of 2^31 elements and more: the first rows and the last ones."""
+    f = _fp8()
+    x, raw = _bf(M, K), torch.empty(E, N, K, device="cuda", dtype=torch.bfloat16).normal_()
+    w, ends = f.fp8_quantize(raw, 128), torch.arange(1, E + 1, device="cuda") * M // E
+    q, y = f.fp8_quantize(x), f.fp8_gemm(x, w, ends)
+    for rows, e in ((slice(0, 20), 0), (slice(M - 20, M), E - 1)):
+        last = f.BlockScaled(q.data[rows], q.scale[rows])
+        _same(last, *_plain(x[rows], 1))
+        expert = f.BlockScaled(w.data[e], w.scale[e])
+        _same(expert, *_plain(raw[e], 128))
+        _product(_dequantized(last), _dequantized(expert), y[rows])

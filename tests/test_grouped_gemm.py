@@ -249,3 +249,21 @@ def test_refusals():
                 (x, torch.zeros(1025, 8, 16, dtype=torch.bfloat16), torch.zeros(1025, dtype=torch.int64))):
         with pytest.raises(ValueError):
             _gg(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,K,N", [(900, 33, 8192, 8192), (280000, 2, 8192, 136), (280000, 2, 136, 8192)])
+def test_more_elements_than_32_bits_count(T, E, K, N):
+    """Weights, rows and results of 2^31 elements and more: the first group's ends and the last one's."""
+    x, w, dy = _bf(T, K), torch.empty(E, N, K, device="cuda", dtype=torch.bfloat16).normal_(std=K ** -0.5), torch.empty(T, N, device="cuda", dtype=torch.bfloat16).normal_()
+    ends = torch.arange(1, E + 1, device="cuda") * (T - 50) // E
+    y, dx, dw = _run(x, w, ends, dy)
+    for e in (0, E - 1):
+        lo, hi = 0 if e == 0 else int(ends[e - 1]), int(ends[e])
+        rows, cols = torch.tensor([lo, hi - 1], device="cuda"), torch.tensor([0, N - 1], device="cuda")
+        a, g, b, d = x[rows].double(), dy[rows].double(), w[e].double(), dy[lo:hi][:, cols].double()
+        _close(y[rows], a @ b.t(), a.abs() @ b.abs().t(), K, f"y of group {e}")
+        _close(dx[rows], g @ b, g.abs() @ b.abs(), N, f"dx of group {e}")
+        a = x[lo:hi].double()
+        _close(dw[e][cols], d.t() @ a, d.abs().t() @ a.abs(), hi - lo, f"dw of group {e}")
+    assert (y[T - 50:] == 0).all() and (dx[T - 50:] == 0).all()

@@ -250,3 +250,20 @@ def test_refusals():
                  (z, tokens, row.clone().requires_grad_(True), row)):
         with pytest.raises(ValueError):
             _loss(*args)
+
+
+@pytest.mark.gpu
+def test_more_logits_than_32_bits_count():
+    rows, vocab = 43000, 50257
+    z = torch.empty(rows, vocab, device="cuda", dtype=torch.bfloat16).normal_().requires_grad_(True)
+    tokens, adv = torch.randint(0, vocab, (rows,), device="cuda"), torch.randn(rows, device="cuda")
+    old, w = torch.full((rows,), -40.0, device="cuda"), torch.ones(rows, device="cuda")          # ratios far above the clamp's end
+    loss, logp = _loss(z, tokens, old, adv, clip=CLIP, reduction="sum")
+    (grad,) = torch.autograd.grad(loss, z)
+    at = torch.cat([torch.arange(40), torch.arange(rows - 40, rows)]).cuda()
+    _, lp, g, c = _formula(z.detach()[at], tokens[at], old[at], adv[at], None, w[at], CLIP, 0.0, False)
+    d = DELTA + 2.0 ** -23 * lp.abs()
+    assert ((logp[at].double() - lp).abs() <= d).all()
+    # c = -r A: its relative error is that of lp, rounded to fp32 twice, beside that of p
+    limit = (HALF_STEP[z.dtype] + 2.0 ** -15 + d[:, None]) * g.abs() + (c.abs() * (2.0 ** -16 + d))[:, None] + LEAST[z.dtype]
+    assert ((grad[at].double() - g).abs() <= limit).all() and (c != 0).any() and (c == 0).any()
