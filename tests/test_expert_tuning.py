@@ -149,3 +149,55 @@ def test_a_decoding_step_replays_from_a_graph():
         x.copy_(torch.randn(1, 128, device="cuda"))
         graph.replay()
         assert torch.equal(out, eight(x))
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream")
+def test_calls_at_once_from_several_threads_and_streams():
+    """Every operator in four threads, each on a stream of its own, forward and backward: the same bits as alone."""
+    import threading
+    from mccl_b200.ops import fp8
+    from mccl_b200.ops.gemm import grouped_gemm, last_error
+    from mccl_b200.ops.loss import fused_policy_loss
+    torch.manual_seed(0)
+
+    def bf(*shape, std=1.0):
+        return (torch.randn(*shape, device="cuda") * std).to(torch.bfloat16)
+
+    shapes = [(3, 4, 520, 776), (900, 8, 264, 520), (5000, 3, 1024, 2048), (40, 6, 2048, 264)]       # tokens, experts, K, N: every form of the products
+    jobs = []
+    for t, e, k, n in shapes:
+        k8 = k // 16 * 16
+        jobs.append(dict(x=bf(t, k).requires_grad_(True), w=bf(e, n, k, std=k ** -0.5).requires_grad_(True), dy=bf(t, n), ends=torch.arange(1, e + 1, device="cuda") * t // e,
+                         x8=bf(t, k8), w8=fp8.fp8_quantize(bf(e, n, k8), 128), one=fp8.fp8_quantize(bf(n, k8), 128), z=bf(t, 5003).requires_grad_(True),
+                         tokens=torch.randint(0, 5003, (t,), device="cuda"), old=torch.full((t,), -9.0, device="cuda"), adv=torch.randn(t, device="cuda")))
+
+    def run(j):
+        y = grouped_gemm(j["x"], j["w"], j["ends"])
+        loss, logp = fused_policy_loss(j["z"], j["tokens"], j["old"], j["adv"])
+        return [y.detach(), *torch.autograd.grad(y, [j["x"], j["w"]], j["dy"]), fp8.fp8_gemm(j["x8"], j["w8"], j["ends"]), fp8.fp8_gemm(j["x8"], j["one"]),
+                loss.detach(), logp, *torch.autograd.grad(loss, j["z"])]
+
+    want = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(me):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for turn in range(40):
+                    i = (me + turn) % len(jobs)
+                    for at, (a, b) in enumerate(zip(run(jobs[i]), want[i])):
+                        if not torch.equal(a, b):
+                            wrong.append((me, turn, i, at))
+        except Exception as error:                                   # a thread's exception would go unseen
+            wrong.append(error)
+
+    threads = [threading.Thread(target=work, args=(me,)) for me in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong[:5]
+    assert last_error() == 0
