@@ -106,8 +106,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
   uint64_t* tmemEmpty = bars + 2 * ST + 2;                 // [ACCS] epilogue -> MMA
   uint64_t* scaleFull = bars + 2 * ST + 4;                 // [kScaleSets] scale warp -> MMA
   uint64_t* scaleEmpty = scaleFull + kScaleSets;           // [kScaleSets] MMA -> scale warp
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(scaleEmpty + kScaleSets);
+  uint64_t* drained = scaleEmpty + kScaleSets;             // after a wait has run out
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* sFail = reinterpret_cast<volatile int*>(tmemSlot + 1);
+  uint32_t* sLoads = tmemSlot + 2;                         // stages the producer has loaded
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int colTiles = (a.N + BN - 1) / BN, kBlocks = (a.K + kBlock - 1) / kBlock;
@@ -117,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
     for (int s = 0; s < ST; ++s) { umma::mbarInit(&full[s], 1); umma::mbarInit(&empty[s], 1); }
     for (int i = 0; i < ACCS; ++i) { umma::mbarInit(&tmemFull[i], 1); umma::mbarInit(&tmemEmpty[i], kEpiWarps); }
     for (int i = 0; i < kScaleSets; ++i) { umma::mbarInit(&scaleFull[i], 1); umma::mbarInit(&scaleEmpty[i], 1); }
+    umma::mbarInit(drained, 1);
     *sFail = 0;
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapA);
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer
-    int stage = 0, e = 0; uint32_t phase = 0;
+    int stage = 0, e = 0; uint32_t phase = 0, loads = 0;
     waitForPredecessor();
     for (int t = blockIdx.x; t < totalTiles && *sFail == 0; t += gridDim.x) {
       Tile tile;
@@ -148,9 +151,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
         umma::mbarExpectTx(&full[stage], S::A_BYTES + S::B_BYTES);
         umma::tmaLoad2d(sA + stage * S::A_BYTES, &a.mapA, &full[stage], kb * kBlock, row);
         grouped::tmaLoad3d(sB + stage * S::B_BYTES, &a.mapB, &full[stage], kb * kBlock, tile.col, tile.e);
+        ++loads;
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
     }
+    *sLoads = loads;
   } else if (warp == 1) {
     // ---------------- MMA issuer: the warp walks the loop together, one thread of it issues
     const bool issues = umma::electOne();
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
         if ((kb & 3) == 0) {
           ok = umma::mbarWait(&scaleFull[set], setPhase, budget);
           umma::tcFenceAfter();
-          if (issues) {
+          if (issues && ok) {
             const uint32_t from = scaleLo0 + (uint32_t)(set * (S::SCALE_BYTES >> 4));
             copyScales(sfa, from, scaleHi);
 #pragma unroll
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
         ok = umma::mbarWait(&full[stage], phase, budget) && ok;
         umma::tcFenceAfter();
         const bool lastOfSet = (kb & 3) == 3 || kb == kBlocks - 1;
-        if (issues) {
+        if (issues && ok) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));
           const uint32_t idesc = instrDesc(BM, BN) + (uint32_t)(kb & 3) * kScaleByte;
           mmaScaled(d, aLo, bLo, hi, idesc, sfa, sfb, kb != 0);
@@ -259,6 +264,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
   waitForPredecessor();                                    // this grid's end stands for its predecessor's too
   umma::tcFenceBefore();
   __syncthreads();
+  if (*sFail != 0) {                                       // the same for all threads
+    if (threadIdx.x == 0) grouped::drainLoads(full, ST, *sLoads);
+    if (warp == 1) grouped::drainProducts(drained);
+    __syncthreads();
+  }
   if (warp == 2) umma::tmemDealloc(tmemBase, gemm::kTmemCols);
 }
 

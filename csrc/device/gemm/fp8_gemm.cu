@@ -71,7 +71,7 @@ mcclResult_t product(const void* x, int64_t ldx, const void* xScale, int64_t ldx
   a.out = static_cast<__nv_bfloat16*>(y);
   a.errFlag = gemm::gemmErrFlag(dev);
   if (a.errFlag == nullptr) return mcclSystemError;
-  a.budgetNs = 2000000000ull;
+  a.budgetNs = gemm::waitNs();
   const int grid = (int)(tiles < sms ? tiles : sms);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return bn == 256 ? launchAs<256>(a, dev, grid, behind, s) : launchAs<128>(a, dev, grid, behind, s);

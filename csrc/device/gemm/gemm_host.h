@@ -16,6 +16,8 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 EncodeTiledFn encodeTiled();
 // The device-visible word in which a GEMM kernel records that it gave up (mcclTpGemmLastError); null where it cannot be had.
 int* gemmErrFlag(int device);
+// How long a wait of a kernel may take: two seconds (mcclDbgGemmWaitNs).
+uint64_t waitNs();
 // Multiprocessors of the current device.
 int gemmSmCount();
 

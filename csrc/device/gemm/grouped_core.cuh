@@ -18,7 +18,8 @@
 //   warp 1      issues the MMAs (one thread); clears the rows behind a group's end
 //   warp 2      allocates and frees tensor memory
 //   warps 4-11  epilogue: four lane quarters x two halves of the columns
-// Every wait is bounded; a role that gives up records it and all roles leave.  No counterpart in the reference.
+// Every wait is bounded; a role that gives up records it, all roles leave, and what is in flight ends before the CTA does (drainLoads and
+// drainProducts).  No counterpart in the reference.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -85,6 +86,23 @@ __device__ __forceinline__ void tmaLoad3d(void* smemDst, const CUtensorMap* map,
 __device__ __forceinline__ void tmaStore3d(const CUtensorMap* map, const void* smemSrc, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                :: "l"(map), "r"(umma::smemAddr(smemSrc)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// After a wait has run out the roles leave their loops with loads and products in flight, which end before the CTA's shared and tensor memory
+// are another's: the loads by the barriers they complete on, the products (and copies of scales) by a commit of the thread that issued
+// them.  With a limit of their own.
+constexpr uint64_t kDrainNs = 1000000000ull;
+// The last loads of `loads` stages in all, one after another.
+__device__ __forceinline__ void drainLoads(uint64_t* full, uint32_t stages, uint32_t loads) {
+  for (uint32_t i = loads > stages ? loads - stages : 0; i < loads; ++i)
+    if (!umma::mbarWait(&full[i % stages], i / stages & 1, kDrainNs)) return;
+}
+// The warp that issued them; its elected thread is the same one every time.
+__device__ __forceinline__ void drainProducts(uint64_t* drained) {
+  if (umma::electOne()) {
+    umma::mmaCommit(drained);
+    umma::mbarWait(drained, 0, kDrainNs);
+  }
 }
 
 // The groups as every role sees them: group e holds the rows [start[e], start[e + 1]); the tiles of all groups up to e number
@@ -268,8 +286,10 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
   uint64_t* empty = bars + ST;                             // [ST] MMA -> TMA
   uint64_t* tmemFull = bars + 2 * ST;                      // [2] MMA -> epilogue
   uint64_t* tmemEmpty = bars + 2 * ST + 2;                 // [2] epilogue -> MMA
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 4);
+  uint64_t* drained = bars + 2 * ST + 4;                   // after a wait has run out
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 5);
   volatile int* sFail = reinterpret_cast<volatile int*>(tmemSlot + 1);
+  uint32_t* sLoads = tmemSlot + 2;                         // stages the producer has loaded
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int colTiles = (a.width + BN - 1) / BN;
@@ -280,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) { umma::mbarInit(&full[s], 1); umma::mbarInit(&empty[s], 1); }
     for (int i = 0; i < 2; ++i) { umma::mbarInit(&tmemFull[i], 1); umma::mbarInit(&tmemEmpty[i], kEpiWarps); }
+    umma::mbarInit(drained, 1);
     *sFail = 0;
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapA);
@@ -309,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer
-    int stage = 0, e = 0; uint32_t phase = 0;
+    int stage = 0, e = 0; uint32_t phase = 0, loads = 0;
     for (int t = blockIdx.x; t < totalTiles && *sFail == 0; t += gridDim.x) {
       Tile tile;
       const int blocks = at(t, &e, &tile);
@@ -332,9 +353,11 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
             for (int c = 0; c < BN / 64; ++c) tmaLoad3d(pb + c * 8192, &a.mapB, &full[stage], tile.col + c * 64, kb * CK, tile.e);
           }
         }
+        ++loads;
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
     }
+    *sLoads = loads;
   } else if (warp == 1) {
     // ---------------- MMA issuer: the warp walks the loop together and clears rows, one thread of it issues
     const bool issues = umma::electOne();
@@ -375,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
           __syncwarp();
         }
         umma::tcFenceAfter();
-        if (issues) {
+        if (issues && ok) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));
           umma::mmaBf16Split(d, aLo, aHi, bLo, bHi, idesc, kb != 0);
           if (!behind || steps > 1) umma::mmaBf16Split(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
@@ -428,6 +451,11 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
   waitForPrevious();
   umma::tcFenceBefore();
   __syncthreads();
+  if (*sFail != 0) {                                       // the same for all threads
+    if (threadIdx.x == 0) drainLoads(full, ST, *sLoads);
+    if (warp == 1) drainProducts(drained);
+    __syncthreads();
+  }
   if (warp == 2) umma::tmemDealloc(tmemBase, gemm::kTmemCols);
 }
 

@@ -52,6 +52,25 @@ __device__ __forceinline__ bool waitWarpCluster(uint64_t* bar, uint32_t parity, 
   *sFail = 1;
   return false;
 }
+__device__ __forceinline__ void storeCluster(void* here, uint32_t cta, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(gemm::umma2::mapToCta(umma::smemAddr(here), cta)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t loadCluster(const void* here, uint32_t cta) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(gemm::umma2::mapToCta(umma::smemAddr(here), cta)) : "memory");
+  return v;
+}
+// The loads in flight after a wait has run out, as in grouped_core.cuh.  Those of both CTAs complete on the leader's barriers, but for a group's last
+// blocks; what the other CTA alone has loaded completes on barriers that the leader has not armed yet.  (A stage that the leader alone has
+// loaded does not complete: there the wait ends by its limit.)
+__device__ __forceinline__ void drainLoads(uint64_t* full, uint64_t* tailFull, const uint32_t* sLoads, int rank) {
+  for (int s = 0; s < ST; ++s)
+    if (!umma::mbarWait(&tailFull[s], (sLoads[1] >> s & 1) ^ 1, grouped::kDrainNs)) return;
+  if (rank != 0) return;
+  uint32_t loads = sLoads[0];
+  for (const uint32_t theirs = loadCluster(sLoads, 1); loads < theirs; ++loads) umma::mbarExpectTx(&full[loads % ST], A_BYTES + B_BYTES);
+  grouped::drainLoads(full, ST, loads);
+}
 
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant__ Args a) {
@@ -70,8 +89,10 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
   uint64_t* tmemEmpty = tmemFull + 2;                      // [2] leader: both CTAs' epilogues have it in registers
   uint64_t* tailFull = tmemEmpty + 2;                      // WEIGHT [ST] each CTA: its loads of a block that reaches behind the group
   uint64_t* tailReady = tailFull + ST;                     // WEIGHT [ST] leader: both CTAs have cleared theirs
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(tailReady + ST);
+  uint64_t* drained = tailReady + ST;                      // each CTA, after a wait has run out
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* sFail = reinterpret_cast<volatile int*>(tmemSlot + 1);
+  uint32_t* sLoads = tmemSlot + 2;                         // stages the producer has loaded, and those of tailFull's next phases (a bit per stage)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)gemm::umma2::clusterCtaRank(), pairIdx = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -83,6 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) { umma::mbarInit(&full[s], 1); umma::mbarInit(&empty[s], 1); umma::mbarInit(&tailFull[s], 1); umma::mbarInit(&tailReady[s], 2); }
     for (int i = 0; i < 2; ++i) { umma::mbarInit(&tmemFull[i], 1); umma::mbarInit(&tmemEmpty[i], 2 * kEpiWarps); }
+    umma::mbarInit(drained, 1);
     *sFail = 0;
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapA);
@@ -113,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer
-    int stage = 0, e = 0; uint32_t phase = 0;
+    int stage = 0, e = 0; uint32_t phase = 0, loads = 0, tailNext = 0;
     for (int t = pairIdx; t < totalTiles && *sFail == 0; t += pairs) {
       Tile tile;
       const int blocks = at(t, &e, &tile);
@@ -125,6 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
         const uint32_t leaderFull = gemm::umma2::mapToCta(umma::smemAddr(&full[stage]), 0);
         if (MODE == WEIGHT && tail && kb == blocks - 1) {  // cleared before the MMAs: complete in this CTA
           if (rank == 0) umma::mbarArrive(&full[stage]);
+          tailNext ^= 1u << stage;
           umma::mbarExpectTx(&tailFull[stage], A_BYTES + B_BYTES);
 #pragma unroll
           for (int c = 0; c < BM / 64; ++c) umma::tmaLoad2d(pa + c * 8192, &a.mapA, &tailFull[stage], tile.row + rank * BM + c * 64, row0 + kb * CK);
@@ -147,9 +170,11 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
             }
           }
         }
+        ++loads;
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
     }
+    sLoads[0] = loads; sLoads[1] = tailNext;
   } else if (warp == 1 && rank == 0) {
     // ---------------- MMA issuer (leader): the warp walks the loop together, one thread of it issues
     const bool issues = umma::electOne();
@@ -175,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
           tailPhase ^= 1u << stage;
         }
         umma::tcFenceAfter();
-        if (issues) {
+        if (issues && ok) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (B_BYTES >> 4));
           mmaBf16(d, aLo, aHi, bLo, bHi, idesc, kb != 0);
           if (!behind || steps > 1) mmaBf16(d, aLo + aStep, aHi, bLo + bStep, bHi, idesc, 1);
@@ -249,7 +274,17 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
   grouped::waitForPrevious();
   umma::tcFenceBefore();
   __syncthreads();
+  if (threadIdx.x == 0 && *sFail != 0) storeCluster(const_cast<int*>(sFail), rank ^ 1, 1);
   gemm::umma2::clusterSync();                              // neither CTA frees tensor memory the other still uses
+  if (*sFail != 0) {                                       // the same for all threads of both
+    if (threadIdx.x == 0) drainLoads(full, tailFull, sLoads, rank);
+    if (warp == 1 && umma::electOne()) {
+      if (rank == 0) commitBoth(drained);
+      umma::mbarWait(drained, 0, grouped::kDrainNs);
+    }
+    __syncthreads();
+    gemm::umma2::clusterSync();
+  }
   if (warp == 2) gemm::umma2::tmemDealloc(tmemBase, gemm::kTmemCols);
 }
 

@@ -95,9 +95,11 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
   uint64_t* sumEmpty = tmemFull + 3;                       // every rank has read this rank's
   uint64_t* scaleFull = tmemFull + 4;                      // [kScaleSets]
   uint64_t* scaleEmpty = scaleFull + fp8::kScaleSets;      // [kScaleSets]
-  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(scaleEmpty + fp8::kScaleSets);
+  uint64_t* drained = scaleEmpty + fp8::kScaleSets;        // after a wait has run out
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* sFail = reinterpret_cast<volatile int*>(tmemSlot + 1);
   int* sGroup = reinterpret_cast<int*>(tmemSlot + 2);      // this group's first row and end, the last group's end
+  uint32_t* sLoads = tmemSlot + 5;                         // stages the producer has loaded
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slices = a.slices, rank = (int)(blockIdx.x % slices), n0 = (int)(blockIdx.x / slices) * BM, e = blockIdx.y;
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
     umma::mbarInit(tmemFull, 1); umma::mbarInit(tmemEmpty, 4);
     umma::mbarInit(sumFull, slices); umma::mbarInit(sumEmpty, slices);
     for (int i = 0; i < fp8::kScaleSets; ++i) { umma::mbarInit(&scaleFull[i], 1); umma::mbarInit(&scaleEmpty[i], 1); }
+    umma::mbarInit(drained, 1);
     *sFail = 0;
     umma::fenceBarrierInit();
     umma::prefetchTensorMap(&a.mapW);
@@ -161,9 +164,10 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer
-    int stage = 0; uint32_t phase = 0;
+    int stage = 0; uint32_t phase = 0, loads = 0;
     waitForPredecessor();
-    for (int64_t r = r0; r < count && *sFail == 0; r += step) {
+    // The first turn whatever another role says: the stages whose weights are requested get their rows.
+    for (int64_t r = r0; r < count && (r == r0 || *sFail == 0); r += step) {
       for (int kb = kb0; kb < kb1; ++kb) {
         if (r != r0 || kb - kb0 >= early) {
           if (!umma::mbarWaitParked(&empty[stage], phase ^ 1, budget)) { *sFail = 1; atomicExch(a.errFlag, 51); break; }
@@ -171,9 +175,11 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
           grouped::tmaLoad3d(sA + stage * S::A_BYTES, &a.mapW, &full[stage], kb * CK, n0, e);
         }
         umma::tmaLoad2d(sB + stage * S::B_BYTES, &a.mapX, &full[stage], kb * CK, first + (int)r);
+        ++loads;
         if (++stage == ST) { stage = 0; phase ^= 1; }
       }
     }
+    *sLoads = loads;
   } else if (warp == 1) {
     // ---------------- MMA issuer: the warp walks the loop together, one thread of it issues
     const bool issues = umma::electOne();
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
         if (FP8 && (kb & 3) == 0) {
           ok = umma::mbarWait(&scaleFull[set], setPhase, budget);
           umma::tcFenceAfter();
-          if (issues) {
+          if (issues && ok) {
             const uint32_t lo = sLo0 + (uint32_t)(set * (S::SCALE_BYTES >> 4));
             fp8::copyScales(sfa, lo, sHi);
             fp8::copyScales(sfb, lo + 32, sHi);
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
         ok = umma::mbarWait(&full[stage], phase, budget) && ok;
         umma::tcFenceAfter();
         const bool lastOfSet = FP8 && ((kb & 3) == 3 || kb == kb1 - 1);
-        if (issues) {
+        if (issues && ok) {
           const uint32_t aLo = aLo0 + (uint32_t)(stage * (S::A_BYTES >> 4)), bLo = bLo0 + (uint32_t)(stage * (S::B_BYTES >> 4));
           if (FP8) {
             const uint32_t idesc = fp8::instrDesc(BM, BT) + (uint32_t)(kb & 3) * fp8::kScaleByte;
@@ -303,6 +309,11 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
   waitForPredecessor();                                    // this grid's end stands for its predecessor's too
   umma::tcFenceBefore();
   __syncthreads();
+  if (*sFail != 0) {                                       // the same for all threads
+    if (threadIdx.x == 0) grouped::drainLoads(full, ST, *sLoads);
+    if (warp == 1) grouped::drainProducts(drained);
+    __syncthreads();
+  }
   gemm::umma2::clusterSync();                              // no rank leaves while another reads its sums
   if (warp == 2) umma::tmemDealloc(tmemBase, S::TMEM);
 }

@@ -90,7 +90,7 @@ mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
   a.out = static_cast<__nv_bfloat16*>(c.out);
   a.errFlag = gemmErrFlag(device);
   if (a.errFlag == nullptr) return mcclSystemError;
-  a.budgetNs = 2000000000ull;
+  a.budgetNs = gemm::waitNs();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return c.fp8 ? launch<true>(bt, a, c, device, nTiles, (int)shares, slices, s) : launch<false>(bt, a, c, device, nTiles, (int)shares, slices, s);
 }

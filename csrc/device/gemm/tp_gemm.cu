@@ -2,6 +2,7 @@
 // argument set-up and launch.  C ABI so the Python layer can call it with raw pointers.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <mutex>
 
 #include "../../comm/comm.h"
@@ -360,6 +361,12 @@ mcclResult_t twoSmGemm(const void* A, const void* B, void* C, void* pre, int M, 
 int* mccl::gemm::gemmErrFlag(int device) { return errFlagFor(device).dev; }
 int mccl::gemm::gemmSmCount() { return smCount(); }
 
+static std::atomic<uint64_t> gWaitNs{0};
+uint64_t mccl::gemm::waitNs() {
+  const uint64_t v = gWaitNs.load(std::memory_order_relaxed);
+  return v != 0 ? v : 2000000000ull;
+}
+
 extern "C" {
 
 // Last error code recorded by a GEMM kernel on the current device (0 = none); reading clears it.
@@ -372,6 +379,9 @@ int mcclTpGemmLastError(void) {
   *f = 0;
   return v;
 }
+
+// How long the waits of the ragged and the 8-bit products launched from now on may take, for tests of what happens then; 0: as ever.
+void mcclDbgGemmWaitNs(uint64_t ns) { gWaitNs.store(ns, std::memory_order_relaxed); }
 
 // Index-arithmetic probe (host only): the (row stripe, column tile) the t-th tile of a GEMM maps to, for
 // mode 0 = plain, 1 = all-gather, 2 = reduce-scatter.  Also reports the tile width the launcher would pick.
