@@ -69,8 +69,7 @@ mcclResult_t product(const void* x, int64_t ldx, const void* xScale, int64_t ldx
   a.ends = ends; a.ends64 = ends64; a.groups = groups;
   a.rows = (int)rows; a.N = N; a.K = K;
   a.out = static_cast<__nv_bfloat16*>(y);
-  a.errFlag = gemm::gemmErrFlag(dev);
-  if (a.errFlag == nullptr) return mcclSystemError;
+  MCCLCHECK(gemm::errorWord(dev, &a.errFlag));
   a.budgetNs = gemm::waitNs();
   const int grid = (int)(tiles < sms ? tiles : sms);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

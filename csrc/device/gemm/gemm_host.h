@@ -14,8 +14,9 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 // cuTensorMapEncodeTiled of the driver; null where it cannot be had.
 EncodeTiledFn encodeTiled();
-// The device-visible word in which a GEMM kernel records that it gave up (mcclTpGemmLastError); null where it cannot be had.
-int* gemmErrFlag(int device);
+// The device-visible word in which a GEMM kernel records that it gave up (mcclTpGemmLastError).  mcclInternalError where one has done so and
+// nobody has read it: what it left unwritten is not built upon.
+mcclResult_t errorWord(int device, int** word);
 // How long a wait of a kernel may take: two seconds (mcclDbgGemmWaitNs).
 uint64_t waitNs();
 // Multiprocessors of the current device.

@@ -96,8 +96,7 @@ bool validRows(const void* p, int64_t ld, int cols) { return p != nullptr && ali
 
 template <int MODE, bool WHOLE = false>
 mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn, bool beside = false) {
-  a.errFlag = gemm::gemmErrFlag(dev);
-  if (a.errFlag == nullptr) return mcclSystemError;
+  MCCLCHECK(gemm::errorWord(dev, &a.errFlag));
   a.budgetNs = gemm::waitNs();
   a.ends = s.ends; a.ends64 = s.ends64; a.groups = s.E; a.rows = (int)s.T;
   const int64_t tiles = rowTiles * ((a.width + bn - 1) / bn);

@@ -70,8 +70,7 @@ mcclResult_t mccl::gemm::pairGemm(const PairCall& c, int device, void* stream) {
   a.contracted = c.mode == DATA ? c.N : c.K;
   a.tileRows = c.N; a.width = width;
   a.out = static_cast<__nv_bfloat16*>(c.out);
-  a.errFlag = gemmErrFlag(device);
-  if (a.errFlag == nullptr) return mcclSystemError;
+  MCCLCHECK(errorWord(device, &a.errFlag));
   a.budgetNs = gemm::waitNs();
   const int grid = (int)std::min<int64_t>(tiles, pairs);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

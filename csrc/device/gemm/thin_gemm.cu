@@ -88,8 +88,7 @@ mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
   a.ends = c.ends; a.ends64 = c.ends64; a.groups = c.groups;
   a.rows = (int)c.rows; a.N = c.N; a.K = c.K; a.slices = slices;
   a.out = static_cast<__nv_bfloat16*>(c.out);
-  a.errFlag = gemmErrFlag(device);
-  if (a.errFlag == nullptr) return mcclSystemError;
+  MCCLCHECK(errorWord(device, &a.errFlag));
   a.budgetNs = gemm::waitNs();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return c.fp8 ? launch<true>(bt, a, c, device, nTiles, (int)shares, slices, s) : launch<false>(bt, a, c, device, nTiles, (int)shares, slices, s);

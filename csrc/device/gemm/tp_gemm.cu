@@ -358,7 +358,15 @@ mcclResult_t twoSmGemm(const void* A, const void* B, void* C, void* pre, int M, 
 
 }  // namespace
 
-int* mccl::gemm::gemmErrFlag(int device) { return errFlagFor(device).dev; }
+mcclResult_t mccl::gemm::errorWord(int device, int** word) {
+  const ErrFlag f = errFlagFor(device);
+  *word = f.dev;
+  if (f.dev == nullptr) return mcclSystemError;
+  const int v = *static_cast<volatile int*>(f.host);
+  if (v == 0) return mcclSuccess;
+  MCCL_WARN("a product launched earlier gave up waiting (code %d): its results are not complete", v);
+  return mcclInternalError;
+}
 int mccl::gemm::gemmSmCount() { return smCount(); }
 
 static std::atomic<uint64_t> gWaitNs{0};

@@ -38,6 +38,12 @@ inline mcclStream_t streamOf(const Tensor& t) {
 inline void check(mcclResult_t rc, const char* what) {
   TORCH_CHECK(rc == mcclSuccess || rc == mcclInProgress, "mccl: ", mcclResultStr(rc), " (code ", (int)rc, "): ", what);
 }
+// For the ragged and the 8-bit products, which refuse while a kernel that gave up has not been heard.
+inline void checkProduct(mcclResult_t rc, const char* what) {
+  TORCH_CHECK(rc != mcclInternalError, "mccl: a product launched earlier on this device gave up waiting and its results are not complete "
+              "(mccl_b200.ops.gemm.last_error() gives the code and clears it): ", what);
+  check(rc, what);
+}
 inline bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
 // Widths at which LayerNorm runs in the library's kernels (FusedLayerNorm and the decoder's nodes alike).  The kernels take
 // others too, in another order of their sums than the tensor library's: a model's results would depend on it.

@@ -91,7 +91,7 @@ py::object fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const T
   const int wide = ends && ends->scalar_type() == at::kLong;
   if (xScale) {
     Tensor xs = scaleRows(*xScale);
-    check(mcclFp8Gemm(rows.data_ptr(), pitchOf(rows), xs.data_ptr(), xs.stride(0), w.data_ptr(), w.stride(-2), ws.data_ptr(), ws.stride(-2), y.data_ptr(), e, wide, (int)E, M,
+    checkProduct(mcclFp8Gemm(rows.data_ptr(), pitchOf(rows), xs.data_ptr(), xs.stride(0), w.data_ptr(), w.stride(-2), ws.data_ptr(), ws.stride(-2), y.data_ptr(), e, wide, (int)E, M,
                       (int)N, (int)K, streamOf(x)), "mcclFp8Gemm");
   } else {
     // One buffer for the quantised rows and, behind them, their scales.  Rows begin at whole lines: a tile's rows of 128 bytes that lie
@@ -100,7 +100,7 @@ py::object fp8Gemm(const Tensor& x, const std::optional<Tensor>& xScale, const T
     const int64_t pitch = blocksOf(K) * kBlock, ld = (blocksOf(K) + 3) / 4 * 4;
     Tensor work = at::empty({M * (pitch + ld)}, x.options().dtype(at::kByte));
     char* q = static_cast<char*>(work.data_ptr());
-    check(mcclFp8GemmBf16Rows(rows.data_ptr(), pitchOf(rows), q, pitch, q + M * pitch, ld, w.data_ptr(), w.stride(-2), ws.data_ptr(), ws.stride(-2), y.data_ptr(), e, wide, (int)E, M,
+    checkProduct(mcclFp8GemmBf16Rows(rows.data_ptr(), pitchOf(rows), q, pitch, q + M * pitch, ld, w.data_ptr(), w.stride(-2), ws.data_ptr(), ws.stride(-2), y.data_ptr(), e, wide, (int)E, M,
                               (int)N, (int)K, streamOf(x)), "mcclFp8GemmBf16Rows");
     counters().gemm += M > 0;
   }

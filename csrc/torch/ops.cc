@@ -216,7 +216,7 @@ py::object gemm(const Tensor& x, const Tensor& w, const std::optional<Tensor>& o
 Tensor groupedForward(const Tensor& x, const Tensor& w, const Tensor& ends) {
   const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(1);
   Tensor y = at::empty({T, N}, x.options());
-  check(mcclGroupedGemm(x.data_ptr(), pitchOf(x), w.data_ptr(), y.data_ptr(), ends.data_ptr(), ends.scalar_type() == at::kLong, (int)E, T, (int)N, (int)K,
+  checkProduct(mcclGroupedGemm(x.data_ptr(), pitchOf(x), w.data_ptr(), y.data_ptr(), ends.data_ptr(), ends.scalar_type() == at::kLong, (int)E, T, (int)N, (int)K,
                         streamOf(x)), "mcclGroupedGemm");
   counters().gemm += T > 0;
   return y;
@@ -243,13 +243,13 @@ struct GroupedFn : torch::autograd::Function<GroupedFn> {
     if (data) ret[0] = at::empty({T, K}, x.options());
     if (weight) ret[1] = at::empty({E, N, K}, w.options());
     if (data && weight) {
-      check(mcclGroupedGemmBackward(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), w.data_ptr(), ret[0].data_ptr(), ret[1].data_ptr(), ends.data_ptr(),
+      checkProduct(mcclGroupedGemmBackward(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), w.data_ptr(), ret[0].data_ptr(), ret[1].data_ptr(), ends.data_ptr(),
                                     wide, (int)E, T, (int)N, (int)K, streamOf(x)), "mcclGroupedGemmBackward");
     } else if (data) {
-      check(mcclGroupedGemmBackwardData(dy.data_ptr(), pitchOf(dy), w.data_ptr(), ret[0].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N, (int)K,
+      checkProduct(mcclGroupedGemmBackwardData(dy.data_ptr(), pitchOf(dy), w.data_ptr(), ret[0].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N, (int)K,
                                         streamOf(x)), "mcclGroupedGemmBackwardData");
     } else if (weight) {
-      check(mcclGroupedGemmBackwardWeight(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), ret[1].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N,
+      checkProduct(mcclGroupedGemmBackwardWeight(dy.data_ptr(), pitchOf(dy), x.data_ptr(), pitchOf(x), ret[1].data_ptr(), ends.data_ptr(), wide, (int)E, T, (int)N,
                                           (int)K, streamOf(x)), "mcclGroupedGemmBackwardWeight");
     }
     counters().gemm += T > 0 ? data + weight : 0;

@@ -23,7 +23,8 @@ mcclResult_t mcclTpGemm(const void* A, const void* B, void* C, int M, int N, int
 mcclResult_t mcclTpGemm2(const void* A, const void* B, void* C, int M, int N, int K, int epilogue, int maxCtas, mcclStream_t stream);
 /* The same by the form the shape allows; pre (nullable, [M, N]): the sums before the activation. */
 mcclResult_t mcclTpGemmKeepPre(const void* A, const void* B, void* C, void* pre, int M, int N, int K, int epilogue, mcclStream_t stream);
-/* Error code the last GEMM kernel on the current device recorded (0 = none); reading clears it. */
+/* Error code the last GEMM kernel on the current device recorded (0 = none); reading clears it.  Until then the products of ragged groups and
+ * the 8-bit products return mcclInternalError: a kernel that gave up waiting has left results unwritten. */
 int mcclTpGemmLastError(void);
 
 /* ---- products of ragged groups of rows (bf16): rows [ends[e-1], ends[e]) of x [rows, K] with w[e] of w [groups, N, K] -------- */

@@ -107,5 +107,7 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.
 
 
 def last_error() -> int:
-    """Error code a GEMM kernel recorded on the current device since the last call (0 = none)."""
+    """Error code a GEMM kernel recorded on the current device since the last call (0 = none): one that waited in vain gives up and leaves its
+    results incomplete.  `grouped_gemm` and `fp8_gemm` raise from then on until this has been called; what a recorded graph replays
+    does not ask."""
     return _lib().mcclTpGemmLastError()

@@ -89,3 +89,24 @@ def test_a_wait_that_runs_out_is_recorded_and_harms_nothing_else(case):
         again = run()
         torch.cuda.synchronize()
         assert last_error() == 0 and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("case", ["few rows", "y, 256 columns", "dw, pairs", "8 bits, 256 columns", "8 bits, few rows in bf16"])
+def test_no_product_follows_one_that_gave_up_unheard(case):
+    from mccl_b200.ops.gemm import last_error
+    torch.manual_seed(0)
+    calls = {c: CASES[c]() for c in {case, "few rows", "y, 128 columns", "dx, 128 columns", "dw, 128 columns", "dx, pairs", "8 bits, 128 columns", "8 bits, few rows"}}
+    want = {c: run() for c, run in calls.items()}
+    torch.cuda.synchronize()
+    with _limit(1):
+        calls[case]()
+    torch.cuda.synchronize()
+    for run in calls.values():
+        for _ in range(2):                                   # raising does not clear it
+            with pytest.raises(RuntimeError, match="last_error"):
+                run()
+    assert last_error() != 0 and last_error() == 0
+    for c, run in calls.items():
+        assert torch.equal(run(), want[c])
+    torch.cuda.synchronize()
+    assert last_error() == 0
