@@ -38,7 +38,7 @@ struct Args {
   int rows, N, K;
   __nv_bfloat16* out;                  // [M, N]
   int* errFlag;
-  uint64_t budgetNs;
+  uint64_t budgetNs, blockNs;          // as in grouped::Args
 };
 
 template <int BN> struct Smem {
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8Kernel(const __grid_constant__
     for (int t = blockIdx.x; t < totalTiles; t += gridDim.x) {
       Tile tile;
       at(t, &e, &tile);
-      if (!grouped::waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 46); break; }
+      if (!grouped::waitWarpLong(&tmemFull[acc], accPhase, budget, kBlocks, a.blockNs, sFail)) { if (lane == 0) atomicExch(a.errFlag, 46); break; }
       umma::tcFenceAfter();
       uint32_t v[COLS];
       const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * 128u + (uint32_t)(half * COLS);

@@ -71,6 +71,7 @@ mcclResult_t product(const void* x, int64_t ldx, const void* xScale, int64_t ldx
   a.out = static_cast<__nv_bfloat16*>(y);
   MCCLCHECK(gemm::errorWord(dev, &a.errFlag));
   a.budgetNs = gemm::waitNs();
+  a.blockNs = gemm::blockNs();
   const int grid = (int)(tiles < sms ? tiles : sms);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return bn == 256 ? launchAs<256>(a, dev, grid, behind, s) : launchAs<128>(a, dev, grid, behind, s);

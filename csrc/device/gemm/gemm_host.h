@@ -17,8 +17,10 @@ EncodeTiledFn encodeTiled();
 // The device-visible word in which a GEMM kernel records that it gave up (mcclTpGemmLastError).  mcclInternalError where one has done so and
 // nobody has read it: what it left unwritten is not built upon.
 mcclResult_t errorWord(int device, int** word);
-// How long a wait of a kernel may take: two seconds (mcclDbgGemmWaitNs).
+// How long a wait of a kernel may take: two seconds, and 20 us for each block of contractions it covers, which take 0.1 to 0.4 us each
+// (mcclDbgGemmWaitNs).
 uint64_t waitNs();
+uint64_t blockNs();
 // Multiprocessors of the current device.
 int gemmSmCount();
 

@@ -46,7 +46,7 @@ struct Args {
   int tileRows, width;                 // WEIGHT: N (rows of an expert's output); columns of the output
   __nv_bfloat16* out;                  // [T, width], or WEIGHT: [E, tileRows, width]
   int* errFlag;
-  uint64_t budgetNs;
+  uint64_t budgetNs, blockNs;          // how long a wait may take, and a block of a contraction that one covers
 };
 
 template <int BN, bool WHOLE> struct Smem {
@@ -178,6 +178,24 @@ template <bool PARKED>
 __device__ __forceinline__ bool waitWarp(uint64_t* bar, uint32_t parity, uint64_t budget, volatile int* sFail) {
   bool ok = *sFail == 0;
   if (ok) ok = PARKED ? umma::mbarWaitParked(bar, parity, budget) : umma::mbarWait(bar, parity, budget);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  *sFail = 1;
+  return false;
+}
+
+// The same for a wait that covers `blocks` blocks of contractions, whose limit grows with them: a long one is no kernel that stands still.  It sees
+// within a microsecond that another role has given up.
+__device__ __forceinline__ bool waitWarpLong(uint64_t* bar, uint32_t parity, uint64_t budget, uint64_t blocks, uint64_t blockNs, volatile int* sFail) {
+  const uint64_t limit = budget + blocks * blockNs;
+  uint64_t t0 = 0;
+  bool ok = false;
+  for (uint32_t spins = 0; *sFail == 0; ++spins) {
+    if (umma::mbarTryWaitParked(bar, parity)) { ok = true; break; }
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    if (spins == 0) t0 = t;
+    else if (t - t0 > limit) break;
+  }
   if (__all_sync(0xffffffffu, ok)) return true;
   *sFail = 1;
   return false;
@@ -428,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupedKernel(const __grid_consta
         clearTile<COLS>(out, limit - r, tile.col + half * COLS, a.width, lane);
         continue;
       }
-      if (!waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 34); break; }
+      if (!waitWarpLong(&tmemFull[acc], accPhase, budget, blocks, a.blockNs, sFail)) { if (lane == 0) atomicExch(a.errFlag, 34); break; }
       umma::tcFenceAfter();
       uint32_t v[COLS];
       const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * 256u + (uint32_t)(half * COLS);

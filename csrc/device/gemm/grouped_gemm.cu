@@ -98,6 +98,7 @@ template <int MODE, bool WHOLE = false>
 mcclResult_t run(Args& a, const Shape& s, int dev, int64_t rowTiles, cudaStream_t stream, int bn, bool beside = false) {
   MCCLCHECK(gemm::errorWord(dev, &a.errFlag));
   a.budgetNs = gemm::waitNs();
+  a.blockNs = gemm::blockNs();
   a.ends = s.ends; a.ends64 = s.ends64; a.groups = s.E; a.rows = (int)s.T;
   const int64_t tiles = rowTiles * ((a.width + bn - 1) / bn);
   if (tiles > INT32_MAX) return mcclInvalidArgument;

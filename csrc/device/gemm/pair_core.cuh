@@ -217,14 +217,17 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
   } else if (warp == 3 && MODE == WEIGHT) {
     // ---------------- of a group's last block, the rows behind its end that the last MMA of 16 takes in (as in grouped_core.cuh)
     int stage = 0, e = 0; uint32_t tailPhase = 0;          // a bit per stage
+    uint64_t walked = 0;                                   // blocks since the last such one
     for (int t = pairIdx; t < totalTiles; t += pairs) {
       Tile tile;
       const int blocks = at(t, &e, &tile), tail = (g.start[tile.e + 1] - g.start[tile.e]) % CK;
       stage = (stage + blocks) % ST;
+      walked += blocks;
       if (tail == 0) continue;
       const int last = (stage + ST - 1) % ST;
-      if (!grouped::waitWarp<true>(&tailFull[last], tailPhase >> last & 1, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 64); break; }
+      if (!grouped::waitWarpLong(&tailFull[last], tailPhase >> last & 1, budget, walked, a.blockNs, sFail)) { if (lane == 0) atomicExch(a.errFlag, 64); break; }
       tailPhase ^= 1u << last;
+      walked = 0;
       uint8_t *pa = sA + last * A_BYTES, *pb = sB + last * B_BYTES;
       for (int i = lane; i < ((tail + 15) / 16 * 16 - tail) * 8; i += 32) {
         const int off = tail * 128 + i * 16;
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) pairKernel(const __grid_constant_
         grouped::clearTile<HALF>(out, limit - r, tile.col + half * HALF, a.width, lane);
         continue;
       }
-      if (!grouped::waitWarp<true>(&tmemFull[acc], accPhase, budget, sFail)) { if (lane == 0) atomicExch(a.errFlag, 66); break; }
+      if (!grouped::waitWarpLong(&tmemFull[acc], accPhase, budget, blocks, a.blockNs, sFail)) { if (lane == 0) atomicExch(a.errFlag, 66); break; }
       umma::tcFenceAfter();
       uint32_t v[HALF];
       const uint32_t from = tmemBase + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * HALF);

@@ -72,6 +72,7 @@ mcclResult_t mccl::gemm::pairGemm(const PairCall& c, int device, void* stream) {
   a.out = static_cast<__nv_bfloat16*>(c.out);
   MCCLCHECK(errorWord(device, &a.errFlag));
   a.budgetNs = gemm::waitNs();
+  a.blockNs = gemm::blockNs();
   const int grid = (int)std::min<int64_t>(tiles, pairs);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return c.mode == FORWARD ? launchAs<FORWARD>(a, device, grid, false, s) : c.mode == DATA ? launchAs<DATA>(a, device, grid, false, s) : launchAs<WEIGHT>(a, device, grid, c.beside, s);

@@ -29,7 +29,7 @@ struct Args {
   int rows, N, K, slices;
   __nv_bfloat16* out;                  // [M, N]
   int* errFlag;
-  uint64_t budgetNs;
+  uint64_t budgetNs, blockNs;          // as in grouped::Args
 };
 
 template <int BT> struct Smem {
@@ -261,11 +261,12 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
     // ---------------- sums: lane quarter q holds 32 of the weights' rows, a column a row of x
     const int q = warp & 3, et = threadIdx.x - 128;
     uint32_t parity = 0;
+    const uint64_t others = budget + (uint64_t)kBlocks * a.blockNs;                  // until another rank's sums are there: its share, and what it waits for
     clusterWait();
     for (int64_t r = r0; r < count; r += step, parity ^= 1) {
-      bool ok = grouped::waitWarp<true>(tmemFull, parity, budget, sFail);
+      bool ok = grouped::waitWarpLong(tmemFull, parity, budget, kb1 - kb0, a.blockNs, sFail);
       if (!ok && lane == 0) atomicExch(a.errFlag, 56);
-      if (ok && r != r0) ok = __all_sync(0xffffffffu, waitCluster(sumEmpty, parity ^ 1, budget));
+      if (ok && r != r0) ok = __all_sync(0xffffffffu, waitCluster(sumEmpty, parity ^ 1, others));
       if (gemm::namedBarrierOr(1, 128, !ok)) { *sFail = 1; break; }      // the four warps meet below: they leave together
       umma::tcFenceAfter();
 #pragma unroll
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 2) thinKernel(const __grid_constant_
       if (lane == 0) umma::mbarArrive(tmemEmpty);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (et < slices) arriveCluster(sumFull, et);
-      ok = __all_sync(0xffffffffu, waitCluster(sumFull, parity, budget));
+      ok = __all_sync(0xffffffffu, waitCluster(sumFull, parity, others));
       if (!ok && lane == 0) atomicExch(a.errFlag, 57);
       if (gemm::namedBarrierOr(1, 128, !ok)) { *sFail = 1; break; }
       // Rank p of the cluster stores the rows p, p + slices, ...: a warp a row, four columns a lane.

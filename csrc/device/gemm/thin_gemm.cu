@@ -90,6 +90,7 @@ mcclResult_t mccl::gemm::thinGemm(const ThinCall& c, int device, void* stream) {
   a.out = static_cast<__nv_bfloat16*>(c.out);
   MCCLCHECK(errorWord(device, &a.errFlag));
   a.budgetNs = gemm::waitNs();
+  a.blockNs = gemm::blockNs();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return c.fp8 ? launch<true>(bt, a, c, device, nTiles, (int)shares, slices, s) : launch<false>(bt, a, c, device, nTiles, (int)shares, slices, s);
 }

@@ -369,11 +369,9 @@ mcclResult_t mccl::gemm::errorWord(int device, int** word) {
 }
 int mccl::gemm::gemmSmCount() { return smCount(); }
 
-static std::atomic<uint64_t> gWaitNs{0};
-uint64_t mccl::gemm::waitNs() {
-  const uint64_t v = gWaitNs.load(std::memory_order_relaxed);
-  return v != 0 ? v : 2000000000ull;
-}
+static std::atomic<uint64_t> gWaitNs{2000000000ull}, gBlockNs{20000};
+uint64_t mccl::gemm::waitNs() { return gWaitNs.load(std::memory_order_relaxed); }
+uint64_t mccl::gemm::blockNs() { return gBlockNs.load(std::memory_order_relaxed); }
 
 extern "C" {
 
@@ -388,8 +386,12 @@ int mcclTpGemmLastError(void) {
   return v;
 }
 
-// How long the waits of the ragged and the 8-bit products launched from now on may take, for tests of what happens then; 0: as ever.
-void mcclDbgGemmWaitNs(uint64_t ns) { gWaitNs.store(ns, std::memory_order_relaxed); }
+// How long the waits of the ragged and the 8-bit products launched from now on may take, and for each block of contractions that one covers, for
+// tests of what happens then.
+void mcclDbgGemmWaitNs(uint64_t ns, uint64_t blockNs) {
+  gWaitNs.store(ns, std::memory_order_relaxed);
+  gBlockNs.store(blockNs, std::memory_order_relaxed);
+}
 
 // Index-arithmetic probe (host only): the (row stripe, column tile) the t-th tile of a GEMM maps to, for
 // mode 0 = plain, 1 = all-gather, 2 = reduce-scatter.  Also reports the tile width the launcher would pick.

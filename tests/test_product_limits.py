@@ -11,17 +11,17 @@ pytestmark = pytest.mark.gpu
 
 
 @contextlib.contextmanager
-def _limit(ns):
-    """Waits of the products launched meanwhile may take so long."""
+def _limit(ns, block_ns=0):
+    """Waits of the products launched meanwhile may take so long, and so much longer for each block of the contractions they cover."""
     import ctypes as C
     from mccl_b200 import _lib
     set_ns = _lib.load().mcclDbgGemmWaitNs
-    set_ns.argtypes, set_ns.restype = [C.c_uint64], None
-    set_ns(ns)
+    set_ns.argtypes, set_ns.restype = [C.c_uint64, C.c_uint64], None
+    set_ns(ns, block_ns)
     try:
         yield
     finally:
-        set_ns(0)
+        set_ns(2_000_000_000, 20_000)
 
 
 def _bf(*shape, std=1.0):
@@ -110,3 +110,30 @@ def test_no_product_follows_one_that_gave_up_unheard(case):
         assert torch.equal(run(), want[c])
     torch.cuda.synchronize()
     assert last_error() == 0
+
+
+LONG = {
+    "few rows": lambda: _grouped([20], 1 << 23, 8, "y"),
+    "y, 128 columns": lambda: _grouped([1] * 300, 1 << 18, 8, "y"),
+    "dx, 128 columns": lambda: _grouped([700], 8, 1 << 18, "dx"),
+    "dw, 128 columns": lambda: _grouped([4000001], 8, 8, "dw"),
+    "dw, few rows an expert": lambda: _grouped([65000] + [0] * 1023, 8, 8, "dw"),
+    "dw, pairs": lambda: _grouped([131072, 65536, 90001], 2048, 4096, "dw"),
+    "8 bits, 128 columns": lambda: _fp8(300, 1 << 19, 8, [1] * 300),
+    "8 bits, few rows": lambda: _fp8(3, 1 << 26, 8),
+}
+
+
+@pytest.mark.parametrize("case", LONG)
+def test_a_contraction_may_take_longer_than_a_wait(case):
+    """The limit is for a kernel that stands still.  A tile's contraction takes 0.2 ms and more here, none of its blocks a hundredth of that."""
+    from mccl_b200.ops.gemm import last_error
+    torch.manual_seed(0)
+    run = LONG[case]()
+    want = run()
+    torch.cuda.synchronize()
+    assert last_error() == 0
+    with _limit(100_000, 20_000):
+        got = run()
+    torch.cuda.synchronize()
+    assert last_error() == 0 and torch.equal(got, want)
