@@ -220,18 +220,23 @@ class ExpertParallelMoE(nn.Module):
 
 
 def _by_expert(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
-    """ops.gemm.grouped_gemm; as separate products where its kernels do not run (which read the ends on the host)."""
-    if x.dtype == w.dtype == torch.bfloat16 and not (x.shape[1] % 8 or w.shape[1] % 8) and may_fuse(x, w, ends):
-        from ..ops.gemm import grouped_gemm
-        return grouped_gemm(x, w, ends)
-    at = [0, *ends.tolist()]
+    """ops.gemm.grouped_gemm where its kernels run.  Elsewhere (other types and widths, more experts, autocast, a trace, a dispatch mode, torch.func)
+    separate products, which read the ends on the host; a trace records them as they are, not their values."""
+    if may_fuse(x, w, ends):
+        from .. import _ext
+        y = _ext.load().grouped_gemm(x, w, ends)
+        if y is not None:
+            return y
+    at = [0, *(ends.unbind() if torch.jit.is_tracing() else ends.tolist())]
     return torch.cat([F.linear(x[a:b], w[e]) for e, (a, b) in enumerate(zip(at, at[1:]))])
 
 
 class DroplessMoE(nn.Module):
     """Top-k routed mixture of experts with all experts on this GPU and no capacity: every token goes to the `top_k` experts with the
     largest router probabilities and is weighted by them (divided by their sum).  The tokens are sorted by expert and the experts are
-    two products over ragged groups (ops/gemm.py), in bf16 on CUDA; nothing is padded or dropped and the host waits for nothing.
+    two products over ragged groups (ops/gemm.py), in bf16 on CUDA; nothing is padded or dropped and the host waits for nothing.  Where
+    those kernels do not run (fp32 parameters under autocast, among others) the experts are separate products, for which the host reads
+    how many tokens each got.
     `quantized()` gives the layer for serving, with the experts in 8 bits."""
 
     def __init__(self, hidden: int, ffn: int, experts: int, top_k: int = 2, device=None, dtype=None):
@@ -271,8 +276,9 @@ class DroplessMoE(nn.Module):
 
 class QuantizedMoE(DroplessMoE):
     """DroplessMoE with its experts in 8 bits with a scale for each block of 128 (ops/fp8.py), for serving: no gradients.  Made by
-    `DroplessMoE.quantized()`; hidden and ffn are multiples of 16, tokens bf16 on CUDA.  The 8-bit experts are neither parameters nor buffers:
-    they stay on their GPU and in no state_dict, which holds the router alone; keep the DroplessMoE's and quantise again."""
+    `DroplessMoE.quantized()`; hidden and ffn are multiples of 16, tokens bf16 on CUDA, at most 1024 experts.  There is no other route: under a
+    trace, a dispatch mode or torch.func it raises.  The 8-bit experts are neither parameters nor buffers: they stay on their GPU and in no
+    state_dict, which holds the router alone; keep the DroplessMoE's and quantise again."""
 
     def __init__(self, layer: DroplessMoE):
         from ..ops.fp8 import fp8_quantize
