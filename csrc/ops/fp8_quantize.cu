@@ -88,13 +88,14 @@ __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat
   }
 }
 
-// One CTA a block of 128 x 128: each thread eight rows' pieces of eight values.
+// One CTA a block of 128 x 128, all of them along the grid's first dimension: each thread eight rows' pieces of eight values.
 __global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloat16* x, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int rows, int K,
-                                                                int rowBlocks) {
+                                                                int rowBlocks, int colBlocks) {
   __shared__ uint32_t warpMax[kThreads / 32];
-  const int rb = (int)(blockIdx.y % rowBlocks);
-  const int64_t outer = blockIdx.y / rowBlocks;
-  const int col = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+  const uint32_t across = blockIdx.x / (uint32_t)colBlocks;
+  const int cb = (int)(blockIdx.x - across * (uint32_t)colBlocks), rb = (int)(across % (uint32_t)rowBlocks);
+  const int64_t outer = across / (uint32_t)rowBlocks;
+  const int col = cb * kBlock + (threadIdx.x & 15) * 8;
   x += outer * rows * K;
   q += outer * rows * ldq;
   uint4 v[8];
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloa
     const int r = rb * kBlock + i * 16 + (threadIdx.x >> 4);
     if (r < rows && col < K) *reinterpret_cast<uint2*>(q + r * ldq + col) = quantize(v[i], byte);
   }
-  if (threadIdx.x == 0) scale[(outer * rowBlocks + rb) * lds + blockIdx.x] = (uint8_t)byte;
+  if (threadIdx.x == 0) scale[(outer * rowBlocks + rb) * lds + cb] = (uint8_t)byte;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -150,16 +151,16 @@ mcclResult_t mcclFp8QuantizeTiles(const void* x, void* q, int64_t ldq, void* sca
   if (outer < 0 || rows <= 0 || K <= 0 || K > INT32_MAX - 256 || rows > INT32_MAX - 256 || K % 16 || ldq < K || ldq % 16 || ldScale < (K + kBlock - 1) / kBlock)
     return mcclInvalidArgument;
   if (outer == 0) return mcclSuccess;
-  const int rowBlocks = (rows + kBlock - 1) / kBlock;
+  const int rowBlocks = (rows + kBlock - 1) / kBlock, colBlocks = (K + kBlock - 1) / kBlock;
   if (!x || !q || !scale || !aligned16(x) || !aligned16(q)) return mcclInvalidArgument;
-  // the grid's second dimension ends at 65535: matrices in turn
-  const int64_t per = rowBlocks <= 65535 ? 65535 / rowBlocks : 0;
+  // a grid ends at 2^31 - 1 blocks: matrices in turn
+  const int64_t each = (int64_t)rowBlocks * colBlocks, per = INT32_MAX / each;
   if (per == 0) return mcclInvalidArgument;
   for (int64_t o = 0; o < outer; o += per) {
     const int64_t n = outer - o < per ? outer - o : per;
-    quantizeTilesKernel<<<dim3((unsigned)((K + kBlock - 1) / kBlock), (unsigned)(n * rowBlocks)), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+    quantizeTilesKernel<<<dim3((unsigned)(n * each)), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
         static_cast<const __nv_bfloat16*>(x) + o * rows * K, static_cast<uint8_t*>(q) + o * rows * ldq, ldq,
-        static_cast<uint8_t*>(scale) + o * rowBlocks * ldScale, ldScale, rows, K, rowBlocks);
+        static_cast<uint8_t*>(scale) + o * rowBlocks * ldScale, ldScale, rows, K, rowBlocks, colBlocks);
   }
   return launchedOk();
 }
