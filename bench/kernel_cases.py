@@ -52,21 +52,31 @@ def timed(fn, launches, warm=2):
     return total / launches
 
 
-def main() -> int:
+SIZES = {"grouped": (2048, 1024), "policy": (50257, None)}     # --n and --k of a case where they are not given
+
+
+def arguments(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["gemm", "grouped", "fp8", "policy", "adamw", "sumsq", "copy", "emu"])
     ap.add_argument("--ranks", type=int, default=8)
     ap.add_argument("--algo", default="twoshot")
     ap.add_argument("--m", type=int, default=8192)
-    ap.add_argument("--n", type=int, default=3584)
-    ap.add_argument("--k", type=int, default=8192)
+    ap.add_argument("--n", type=int)
+    ap.add_argument("--k", type=int)
     ap.add_argument("--experts", type=int, default=8)
     ap.add_argument("--elems", type=int, default=0)
     ap.add_argument("--mbytes", type=int, default=512)
     ap.add_argument("--launches", type=int, default=3)
     ap.add_argument("--cublas", action="store_true", help="gemm: also time torch.matmul (cuBLAS) on the same operands")
     ap.add_argument("--two-sm", action="store_true", help="gemm: the form in which pairs of SMs share a 256-row tile")
-    args = ap.parse_args()
+    args = ap.parse_args(argv)
+    n, k = SIZES.get(args.case, (3584, 8192))
+    args.n, args.k = n if args.n is None else args.n, k if args.k is None else args.k
+    return args
+
+
+def main() -> int:
+    args = arguments()
     torch.cuda.set_device(0)
     dev = torch.device("cuda", 0)
     hbm, tflops, src = peaks()
@@ -111,7 +121,7 @@ def main() -> int:
                     "with_quantisation_us": round(both * 1e3, 1), "kernel_error": G.last_error()})
     elif args.case == "policy":
         from mccl_b200.ops.loss import fused_policy_loss
-        rows, vocab = args.m, args.n if args.n != 3584 else 50257
+        rows, vocab = args.m, args.n
         z = torch.randn(rows, vocab, device=dev).to(torch.bfloat16)
         a, old, adv = torch.randint(0, vocab, (rows,), device=dev), torch.full((rows,), -11.0, device=dev), torch.randn(rows, device=dev)
         with torch.no_grad():
