@@ -52,6 +52,16 @@ def timed(fn, launches, warm=2):
     return total / launches
 
 
+def policy_inputs(rows, vocab, dev):
+    """Logits and the rest of a policy loss with a KL term: every row has a gradient.  (The backward pass does not read a row that has none, of weight
+    zero or held by the clamp: three passes over the logits would not be what it moves.)"""
+    z = torch.randn(rows, vocab, device=dev).to(torch.bfloat16)
+    tokens = torch.randint(0, vocab, (rows,), device=dev)
+    now = torch.cat([a.float().log_softmax(1).gather(1, t[:, None])[:, 0] for a, t in zip(z.split(1024), tokens.split(1024))])
+    return z, dict(tokens=tokens, old_logp=now + 0.2 * torch.randn(rows, device=dev), ref_logp=now + 0.5 * torch.randn(rows, device=dev),
+                   advantages=torch.randn(rows, device=dev), kl_coef=0.04)
+
+
 SIZES = {"grouped": (2048, 1024), "policy": (50257, None)}     # --n and --k of a case where they are not given
 
 
@@ -122,12 +132,11 @@ def main() -> int:
     elif args.case == "policy":
         from mccl_b200.ops.loss import fused_policy_loss
         rows, vocab = args.m, args.n
-        z = torch.randn(rows, vocab, device=dev).to(torch.bfloat16)
-        a, old, adv = torch.randint(0, vocab, (rows,), device=dev), torch.full((rows,), -11.0, device=dev), torch.randn(rows, device=dev)
+        z, terms = policy_inputs(rows, vocab, dev)
         with torch.no_grad():
-            fwd = timed(lambda: fused_policy_loss(z, a, old, adv), args.launches)
+            fwd = timed(lambda: fused_policy_loss(z, **terms), args.launches)
         zr = z.requires_grad_(True)
-        both = timed(lambda: torch.autograd.grad(fused_policy_loss(zr, a, old, adv)[0], zr), args.launches)
+        both = timed(lambda: torch.autograd.grad(fused_policy_loss(zr, **terms)[0], zr), args.launches)
         out.update({"rows": rows, "vocab": vocab, "forward_us": round(fwd * 1e3, 1), "with_gradient_us": round(both * 1e3, 1),
                     "gbs": round(6 * rows * vocab / both / 1e6, 1), "frac_of_copy_peak": round(6 * rows * vocab / both / 1e6 / hbm, 3)})
     elif args.case == "adamw":

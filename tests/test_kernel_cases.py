@@ -20,3 +20,13 @@ def cases():
 def test_a_size_that_is_given_is_the_one_measured(cases, argv, n, k):
     args = cases.arguments(argv.split())
     assert (args.n, args.k) == (n, k)
+
+
+@pytest.mark.gpu
+def test_every_row_of_the_policy_loss_is_read_and_written(cases):
+    import torch
+    from mccl_b200.ops.loss import fused_policy_loss
+    torch.manual_seed(0)
+    z, terms = cases.policy_inputs(3000, 257, torch.device("cuda"))
+    (g,) = torch.autograd.grad(fused_policy_loss(z.requires_grad_(True), **terms)[0], z)
+    assert (g != 0).any(1).all()
