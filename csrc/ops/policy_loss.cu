@@ -199,8 +199,9 @@ __global__ void __launch_bounds__(kRowThreads) policyRowsKernel(const T* logits,
     clusterMeet();                             // no CTA leaves before its sums have been read
   }
   if (threadIdx.x != 0 || blockIdx.x != 0) return;
-  const double over = !mean ? 1. : sumW == 0. ? 0. : 1. / sumW;
-  *loss = over == 0. ? 0.f : (float)(sumL * over);
+  const bool none = mean && sumW == 0.;
+  const double over = none ? 0. : mean ? 1. / sumW : 1.;
+  *loss = none ? 0.f : (float)(sumL * over);   // weights that add up to infinity: NaN
   *inverse = (float)over;
 }
 
