@@ -90,7 +90,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 struct Shape { const void* ends; int ends64, E; int64_t T; int N, K; };
 
 bool valid(const Shape& s) {
-  return s.ends != nullptr && s.E > 0 && s.E <= kMaxGroups && s.T >= 0 && s.T <= INT32_MAX - 256 && s.N > 0 && s.K > 0 && s.N % 8 == 0 && s.K % 8 == 0;
+  return s.ends != nullptr && s.E > 0 && s.E <= kMaxGroups && s.T >= 0 && s.T <= INT32_MAX - 256 && s.N > 0 && s.K > 0 && s.N <= INT32_MAX - 256 && s.K <= INT32_MAX - 256 &&
+         s.N % 8 == 0 && s.K % 8 == 0;
 }
 bool validRows(const void* p, int64_t ld, int cols) { return p != nullptr && aligned16(p) && ld >= cols && ld % 8 == 0; }
 

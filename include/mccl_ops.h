@@ -31,7 +31,7 @@ int mcclTpGemmLastError(void);
 /* y[t] = x[t] w[e]^T; dx[t] = dy[t] w[e]; dw[e] = sum over the group of dy[t]^T x[t].  ends: on the device, int32 or (ends64) int64,
  * read as the largest so far within [0, rows]; rows behind the last end are zero in y and dx and no part of dw.  N and K multiples of 8,
  * pointers 16-byte aligned, x and dy with rows ld elements apart (a multiple of 8), the rest contiguous; at most
- * mcclGroupedGemmMaxGroups() groups. */
+ * mcclGroupedGemmMaxGroups() groups; rows, N and K at most 2^31 - 257. */
 int          mcclGroupedGemmMaxGroups(void);
 mcclResult_t mcclGroupedGemm(const void* x, int64_t ldx, const void* w, void* y, const void* ends, int ends64, int groups, int64_t rows, int N,
                              int K, mcclStream_t stream);
