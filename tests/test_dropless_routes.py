@@ -147,3 +147,27 @@ def test_more_experts_than_the_kernels_take(experts, kernels):
     ref = torch.autograd.grad(want, [xr, wi, wo], dy.double())
     assert _rel(y, want) <= 6 * U
     assert _rel(got[1], ref[1]) <= 12 * U and _rel(got[2], ref[2]) <= 12 * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 9, 300, 3000])
+def test_quantised_layer_against_64_bits_on_its_own_operands(tokens):
+    """The operands are the quantised ones, so what is left are the second product's fp32 sums (a step for each addition, as in tests/test_fp8.py) and
+    three roundings to bf16: that product's, its product's with the weight, the sum's.  Their products with one another are below a hundredth."""
+    from mccl_b200.ops import fp8
+    layer, x, _ = _gpu(tokens)
+    eight = layer.quantized()
+    weight, expert = layer.route(x)
+    by_expert, order = expert.reshape(-1).sort(stable=True)
+    sizes = torch.bincount(by_expert, minlength=6)
+    h = F.silu(fp8.fp8_gemm(x.repeat_interleave(2, 0)[order], eight.w_in, sizes.cumsum(0)))     # the same rows in the same kernel: the same bits
+    h, w = fp8.fp8_quantize(h).dequantize().double(), eight.w_out.dequantize().double()
+
+    def by_token(h, w):
+        rows = torch.empty(2 * tokens, 128, device="cuda", dtype=torch.float64)
+        rows[order] = torch.cat([a @ w[e].t() for e, a in enumerate(h.split(sizes.tolist()))])
+        return rows.view(tokens, 2, 128) * weight.double()[..., None]
+    parts, most = by_token(h, w), by_token(h.abs(), w.abs()).sum(1)
+    want = parts.sum(1)
+    limit = 1.01 * (U * (2 * parts.abs().sum(1) + want.abs()) + 2 * 272 * 2.0 ** -24 * most)
+    assert ((eight(x).double() - want).abs() <= limit).all()
