@@ -20,7 +20,8 @@ BLOCK = 128
 class BlockScaled(NamedTuple):
     """`data` (float8_e4m3fn, [..., M, K]) and the scale of each block (float8_e8m0fnu, [..., M / rows, K / 128] rounded up), rows being
     1 or 128.  `fp8_quantize` keeps the rows of the scales a multiple of four bytes apart, as the kernels read them, and the rows of weights a
-    multiple of 128; scales of another pitch, and values whose rows are not a multiple of 16 bytes apart, are copied in every call."""
+    multiple of 128; scales of another pitch, and values whose elements are not adjacent or whose rows are not a multiple of 16 bytes apart,
+    are copied in every call."""
     data: torch.Tensor
     scale: torch.Tensor
 

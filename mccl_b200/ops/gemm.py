@@ -91,7 +91,9 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.
     bf16 x [T, K] and w [E, N, K] (an nn.Linear weight for each expert), K and N multiples of 8; `ends` [E] int32 or int64 on the
     device, e.g. the cumulative sum of the tokens per expert: the host never waits for it.  An end below an earlier one is read as
     that one, one outside [0, T] as the nearest.  Rows from ends[-1] on belong to no expert: they are zero in y and in x's gradient
-    and no part of w's; the gradient of an expert without rows is zero."""
+    and no part of w's; the gradient of an expert without rows is zero.  Weights that are a view with gaps or in another order (half of a
+    joined matrix, a transposed one) are copied in every call, and so are rows whose elements are not adjacent or that are not a multiple of 16
+    bytes apart."""
     y = _ext.load().grouped_gemm(x, w, ends) if x.is_cuda else None
     if y is not None:
         return y
