@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(kThreads) quantizeRowsKernel(const __nv_bfloat
   }
 }
 
-// One CTA a block of 128 x 128, all of them along the grid's first dimension: each thread eight rows' pieces of eight values.
+// One CTA a block of 128 x 128, all of them along the grid's first dimension: each thread eight rows' pieces of eight values.  8192 x 8192 41 us,
+// 4.9 TB/s; 3584 x 8192 20.5 us.
 __global__ void __launch_bounds__(kThreads) quantizeTilesKernel(const __nv_bfloat16* x, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int rows, int K,
                                                                 int rowBlocks, int colBlocks) {
   __shared__ uint32_t warpMax[kThreads / 32];

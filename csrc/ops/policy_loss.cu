@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t atRank(const void* here, int rank) {
 
 // stats[row], stats[rows + row] = maximum and sum of exp(x - maximum).  gridDim.y CTAs share a row, as one cluster: each leaves its pair in
 // its shared memory, and the first adds them up rank by rank.
-// Instructions bound it beside memory: 8192 x 50257 bf16 with the rows' terms 144 us, 5.7 TB/s; 170 us where the distance of a thread's pieces is
+// Instructions bound it beside memory: 8192 x 50257 bf16 with the rows' terms 147 us, 5.6 TB/s; 170 us where the distance of a thread's pieces is
 // no constant, hence SHARED (whether there are several CTAs).
 template <class T, int U, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 6) policyForwardKernel(const T* logits, int64_t rows, int64_t ld, int vocab, float* stats) {
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kRowThreads) policyRowsKernel(const T* logits,
 template <class T> __device__ __forceinline__ float gradExp(float x) { return __expf(x); }
 template <> __device__ __forceinline__ float gradExp<float>(float x) { return expf(x); }
 
-// Bound by memory: 8192 x 50257 bf16 250 us, 6.5 TB/s.  blockIdx.y: which slice of the row.  SAME: a row's 16-byte boundaries lie at the same elements in the logits and in the gradient.
+// Bound by memory: 8192 x 50257 bf16, every row read, 258 us, 6.4 TB/s; with a tenth of the rows of weight zero 248 us, 6.3 TB/s.  blockIdx.y: which slice of the row.  SAME: a row's 16-byte boundaries lie at the same elements in the logits and in the gradient.
 template <class T, int U, bool SAME>
 __global__ void __launch_bounds__(kThreads) policyBackwardKernel(const T* logits, int64_t rows, int64_t ld, T* grad, int64_t gradLd, int vocab, int width,
                                                                  const int64_t* tokens, const float* stats, const float* gradOut,
