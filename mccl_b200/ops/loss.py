@@ -39,7 +39,8 @@ def fused_policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torc
     weights x terms, with `reduction="mean"` over the sum of the weights (zero, with a zero gradient, where that is zero).  A row of
     weight zero takes no part whatever it holds (padding); one of another weight whose token is outside the vocabulary makes the loss
     NaN.  The last KL factor needs `ref_logp`.  Per row: int64 `tokens`, fp32 `old_logp`, `advantages`, `ref_logp`, and `weights`
-    in fp32 or bool; they are constants and must not ask for a gradient.  Columns from `vocab` on are padding.  Differentiable in
+    in fp32 or bool; they are constants and must not ask for a gradient.  With "mean" the weights add up to 2^-126 at
+    least, or to zero: the gradient's divisor is fp32.  Columns from `vocab` on are padding.  Differentiable in
     the logits, which stay as they are (the gradient has memory of its own); once only."""
     if reduction not in ("mean", "sum"):
         raise ValueError(f"fused_policy_loss: reduction is 'mean' or 'sum' (got {reduction!r})")
